@@ -10,6 +10,14 @@ same signatures, same wire format (version 2, byte-identical updates), same all-
   update exists, and a wrong cache produces an update the receiver rejects, never wrong weights.
 - Receiver: ``checksums`` maps name -> (checksum, tensor._version); a cached checksum is used
   only while the tensor's ``_version`` is unchanged since this library last wrote it.
+Beside it stands what a trainer does between its backward pass and ``encode_update`` (trainer.py,
+no counterpart in the reference):
+
+    loss = policy_loss(logits, tokens, advantages, old_logp=old, ref_logp=ref, mask=mask, kl_coef=0.04).loss
+    loss.backward()
+    adamw_step(masters, grads, exp_avg, exp_avg_sq, cur, lr=1e-6, step=t, norm=grad_norm(grads), max_norm=1.0)
+    update = encode_update(prev, cur, send_chk)
+
 All arithmetic runs in hand-written CUDA kernels (libcrukx_b200.so, C ABI in
 include/crukx_b200.h); there is no CPU implementation and no other backend.
 """
@@ -23,9 +31,11 @@ from dataclasses import dataclass
 import torch
 
 from . import codec
+from .trainer import PolicyLoss, adamw_step, clip_grads, grad_norm, policy_loss
 from .wire import CorruptUpdate, encoder_parse, parse, parse_device, serialize
 
-__all__ = ["encode_update", "apply_update", "encode_update_device", "UpdateStats", "CorruptUpdate"]
+__all__ = ["encode_update", "apply_update", "encode_update_device", "UpdateStats", "CorruptUpdate",
+           "policy_loss", "PolicyLoss", "grad_norm", "clip_grads", "adamw_step"]
 
 
 @dataclass

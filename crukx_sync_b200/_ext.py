@@ -27,7 +27,8 @@ EXPORTS = [
     "crx_encode_device", "crx_encoded_copy_device", "crx_parse_head", "crx_parse_device",
     "crx_encode_global", "crx_encoded_part", "crx_encoded_part_copy", "crx_apply_versioned",
     "crx_ctx_hist_cache_hits", "crx_alloc_calls", "crx_size_stats", "crx_apply_to_host",
-    "crx_ctx_kernel_gaps", "crx_encoded_parse_device",
+    "crx_ctx_kernel_gaps", "crx_encoded_parse_device", "crx_grads_workspace", "crx_grad_norm", "crx_clip_grads",
+    "crx_adamw_step", "crx_policy_workspace", "crx_policy_loss", "crx_policy_backward",
 ]
 
 # collective callbacks of crx_encode_global
@@ -100,6 +101,13 @@ def load():
             "crx_apply_to_host": ([P, P, P, P, P, P, P, P, CP, SZ], ctypes.c_int),
             "crx_ctx_kernel_gaps": ([P, CP, SZ, P, I32], I32),
             "crx_encoded_parse_device": ([P, P, ctypes.POINTER(P), CP, SZ], ctypes.c_int),
+            "crx_grads_workspace": ([I32], I64),
+            "crx_grad_norm": ([I32, P, P, P, P, I64, P, P, CP, SZ], ctypes.c_int),
+            "crx_clip_grads": ([I32, P, P, P, P, ctypes.c_float, P, P, I64, P, P, CP, SZ], ctypes.c_int),
+            "crx_adamw_step": ([I32, P, P, P, P, P, P, P, CP, P, CP, SZ], ctypes.c_int),
+            "crx_policy_workspace": ([I64, I64], I64),
+            "crx_policy_loss": ([CP, P, CP, SZ], ctypes.c_int),
+            "crx_policy_backward": ([CP, P, I32, P, CP, SZ], ctypes.c_int),
         }
         for name, (args, res) in sig.items():
             fn = getattr(L, name)

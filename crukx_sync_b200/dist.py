@@ -192,6 +192,22 @@ def partition_contiguous(numels: Sequence[int], world: int) -> list[tuple[int, i
     return [(bounds[k], bounds[k + 1]) for k in range(world)]
 
 
+def grad_norm_global(grads: Mapping[str, torch.Tensor], group=None) -> torch.Tensor:
+    """The norm of all ranks' gradients together, each rank passing the ones it owns (see partition):
+    a 0-d fp32 tensor, the same on every rank, for clip_grads(norm=...) and adamw_step(norm=...).
+    One all-reduce of one double: squares of an fp32 norm neither overflow nor underflow there."""
+    import torch.distributed as td
+
+    from . import trainer
+
+    norm = trainer.grad_norm(grads)
+    if not td.is_initialized() or td.get_world_size(group) == 1:
+        return norm
+    square = norm.double().square()
+    td.all_reduce(square, group=group)
+    return square.sqrt().float()
+
+
 _PART_KEYS = ("prefix", "tensors", "table", "payload")
 
 

@@ -258,6 +258,82 @@ int crx_checksum_noalloc(const int16_t* data, int64_t n, void* stream, uint64_t*
 int crx_size_stats(crx_ctx* ctx, int32_t n_tensors, const int16_t* const* prev, const int16_t* const* cur,
                    const int64_t* numel, void* stream, uint64_t* out, char* err, size_t errlen);
 
+/*
+ * The trainer's side of a sync step (no reference counterpart: the reference starts at the two
+ * weight dicts).  These entry points take no context, allocate nothing, never synchronise and keep
+ * nothing between calls: scratch is the caller's, so calls may run on any streams at once and be
+ * captured into graphs.  Device pointers belong to the current device; host scalars are baked into
+ * a captured graph.  Element types of gradients and logits:
+ */
+#define CRX_BF16 0
+#define CRX_FP16 1
+#define CRX_FP32 2
+
+/* Bytes of device scratch (8-byte aligned) that crx_grad_norm and crx_clip_grads need. */
+int64_t crx_grads_workspace(int32_t n_tensors);
+/* *norm (device, fp32) = sqrt of the sum of squares over all elements of n gradients.  Squares are
+ * summed so that neither overflow nor underflow of fp32 squares shows in the result; the order of
+ * the sum is fixed, so equal calls give equal bits. */
+int crx_grad_norm(int32_t n_tensors, const void* const* grads, const int32_t* dtypes, const int64_t* numel, void* workspace,
+                  int64_t workspace_bytes, float* norm, void* stream, char* err, size_t errlen);
+/* out[i] = c * grads[i], c = min(1, max_norm / (norm + 1e-6)), rounded to the gradient's type.  The
+ * norm is *norm_in (device), or, where that is NULL, the one of these gradients; norm_out (NULL
+ * only with norm_in) receives it.  out[i] is grads[i] itself or memory of its own: tensors that
+ * overlap otherwise are CRX_VALUE_ERROR, nothing launched.  With out[i] == grads[i] and c = 1
+ * nothing is written. */
+int crx_clip_grads(int32_t n_tensors, const void* const* grads, void* const* out, const int32_t* dtypes, const int64_t* numel,
+                   float max_norm, const float* norm_in, void* workspace, int64_t workspace_bytes, float* norm_out,
+                   void* stream, char* err, size_t errlen);
+
+typedef struct crx_adamw_args {
+    double lr, beta1, beta2, eps, weight_decay;
+    int64_t step;            /* of this update, from 1 */
+    const float* lr_p;       /* device; not NULL: read in place of lr when the kernel runs */
+    const int64_t* step_p;   /* device; not NULL: read in place of step */
+    const float* norm;       /* device; not NULL: the gradients' norm.  Where it is not finite, masters and moments stay */
+    float max_norm;          /* > 0: gradients are scaled by min(1, max_norm / (*norm + 1e-6)) on the way */
+} crx_adamw_args;
+/* AdamW with decoupled weight decay on fp32 masters and moments, in place; weights[i] (weights may
+ * be NULL) receives the bf16 rounding of master i.  Memory that is written may not be shared. */
+int crx_adamw_step(int32_t n_tensors, float* const* master, const void* const* grads, const int32_t* dtypes,
+                   float* const* exp_avg, float* const* exp_avg_sq, void* const* weights, const int64_t* numel,
+                   const crx_adamw_args* args, void* stream, char* err, size_t errlen);
+
+/* A [batch, steps] array of per-token values on the device; strides in elements, 0 to broadcast. */
+typedef struct crx_rows {
+    const void* p;
+    int64_t stride_b, stride_t;
+} crx_rows;
+typedef struct crx_policy_args {
+    int64_t batch, steps, vocab;
+    crx_rows logits, grad;      /* row starts; the vocabulary is contiguous.  grad.p NULL: no gradient */
+    crx_rows tokens, advantages;
+    crx_rows old_logp, ref_logp, mask;   /* p NULL: none */
+    float* logp;                /* [batch, steps] */
+    float* loss;
+    float* stats;               /* 2: KL, clipped fraction */
+    float* rows;                /* crx_policy_workspace bytes, 16-byte aligned; crx_policy_backward reads them */
+    double denom;               /* 0: the sum of the mask */
+    float clip_low, clip_high, kl_coef, temperature;
+    int32_t dtype;              /* of logits and grad */
+    int32_t tokens64;           /* tokens are int64, else int32 */
+    int32_t mask_f32;           /* mask is fp32 weights, else one byte per token */
+    int32_t pad;
+} crx_policy_args;
+int64_t crx_policy_workspace(int64_t batch, int64_t steps);
+/* Clipped policy loss with a KL term over batch * steps tokens; with grad.p, the gradient of the
+ * loss to the logits too, from the same pass.  Per token with mask w != 0:
+ *   logp = z[token] - logsumexp(z), z = logits / temperature;  r = exp(logp - old_logp)  (none: 1)
+ *   l = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^x - x - 1), x = ref_logp - logp
+ * loss = sum w l / denom; KL and clipped fraction are averaged the same way.  Tokens with w = 0 are
+ * left out whatever their values: logp 0, gradient 0, logits not read.  denom = 0 in effect (an
+ * all-zero mask) gives 0.  A token outside the vocabulary where w != 0 makes the loss NaN. */
+int crx_policy_loss(const crx_policy_args* args, void* stream, char* err, size_t errlen);
+/* grad = scale * the gradient that crx_policy_loss wrote (args as it got them; scale: device
+ * scalar).  unless_one != 0: nothing is done where *scale is 1 (grad holds the answer already). */
+int crx_policy_backward(const crx_policy_args* args, const float* scale, int32_t unless_one, void* stream, char* err,
+                        size_t errlen);
+
 #ifdef __cplusplus
 }
 #endif
