@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 import struct
 from collections.abc import Mapping
 from contextlib import nullcontext
@@ -31,6 +32,7 @@ from . import _ext
 from .codec import _cuda_device, _raise
 
 _CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # CRX_BF16, CRX_FP16, CRX_FP32
+_GRADS, _F32, _BF16 = frozenset(_CODES), frozenset([torch.float32]), frozenset([torch.bfloat16])
 _GRAD_TYPES = "bfloat16, float16 or float32"
 
 
@@ -52,34 +54,49 @@ def _check(name: str, t, dtypes, what: str) -> None:
         raise ValueError(f"{name}: expected a CUDA tensor")
 
 
+_T = torch.Tensor
+_dtype_of = operator.attrgetter("dtype")
+
+
 def _gather(what: str, tensors: Mapping, dtypes, types: str, index: int | None):
-    """The dict's tensors, checked, and the index of their one device."""
+    """The dict's tensors, checked, their addresses, element counts and types, and the index of
+    their one device.  Whole-list calls: a model has hundreds of tensors and the step waits for this."""
     if not isinstance(tensors, Mapping):
         raise ValueError(f"{what} must be a dict of name -> tensor, got {type(tensors)}")
     out = list(tensors.values())
-    T = torch.Tensor
-    for t in out:
-        if not isinstance(t, T) or t.dtype not in dtypes or not t.is_cuda or t.layout != torch.strided or not t.is_contiguous():
-            for name, x in tensors.items():
-                _check(name, x, dtypes, types)
-        d = t.get_device()
-        if index is None:
-            index = d
-        elif d != index:
-            raise ValueError("all tensors must be on one device")
-    return out, index
+    try:
+        types_of = list(map(_dtype_of, out))
+        kinds = set(types_of)
+        devices = set(map(_T.get_device, out))
+        fine = kinds <= dtypes and -1 not in devices and all(map(_T.is_contiguous, out))
+        if fine:
+            ptrs, numels = list(map(_T.data_ptr, out)), list(map(_T.numel, out))
+    except (TypeError, AttributeError, RuntimeError, NotImplementedError):   # not tensors, or not strided ones
+        fine = False
+    if not fine:
+        for name, t in tensors.items():
+            _check(name, t, dtypes, types)
+        raise ValueError(f"{what}: expected contiguous {types} CUDA tensors")
+    if index is not None:
+        devices.add(index)
+    if len(devices) > 1:
+        raise ValueError("all tensors must be on one device")
+    codes = [_CODES[kinds.pop()]] * len(out) if len(kinds) == 1 else list(map(_CODES.__getitem__, types_of))
+    return out, ptrs, numels, codes, next(iter(devices), None)
 
 
 def _match(what: str, tensors: Mapping, names, numels, dtypes, types: str, index: int):
-    """`tensors` under the same names and sizes, in the order of `names`."""
+    """`tensors` under the same names and sizes, in the order of `names`: (tensors, addresses, types)."""
     if not isinstance(tensors, Mapping) or tensors.keys() != names:
         odd = sorted(set(tensors) ^ set(names))[:5] if isinstance(tensors, Mapping) else type(tensors)
         raise ValueError(f"{what} and the gradients differ in tensor names: {odd}")
-    out, _ = _gather(what, {n: tensors[n] for n in names}, dtypes, types, index)
-    for name, t, n in zip(names, out, numels):
-        if t.numel() != n:
-            raise ValueError(f"{name}: {what} and the gradient differ in shape")
-    return out
+    if list(tensors) != list(names):
+        tensors = {n: tensors[n] for n in names}
+    out, ptrs, n, codes, _ = _gather(what, tensors, dtypes, types, index)
+    if n != numels:
+        name = next(name for name, a, b in zip(names, n, numels) if a != b)
+        raise ValueError(f"{name}: {what} and the gradient differ in shape")
+    return out, ptrs, codes
 
 
 def _scalar(what: str, t, dtype, index: int) -> None:
@@ -91,16 +108,12 @@ def _no_tensors() -> int:
     return _cuda_device(torch.device("cuda")).index
 
 
-def _ptrs(tensors):
-    return _ext.ptr_array([t.data_ptr() for t in tensors])
-
-
 def grad_norm(grads: Mapping[str, torch.Tensor]) -> torch.Tensor:
     """sqrt(sum of g^2) over every element of every gradient, as a 0-d fp32 CUDA tensor.
 
     bf16, fp16 and fp32 gradients may be mixed.  The sum is held in 64 bits and squares that would
     overflow or vanish in fp32 count in full; its order is fixed, so equal gradients give equal bits."""
-    tensors, index = _gather("gradients", grads, _CODES, _GRAD_TYPES, None)
+    tensors, ptrs, numels, codes, index = _gather("gradients", grads, _GRADS, _GRAD_TYPES, None)
     if index is None:
         index = _no_tensors()
     L = _ext.load()
@@ -110,9 +123,8 @@ def grad_norm(grads: Mapping[str, torch.Tensor]) -> torch.Tensor:
         norm = torch.empty((), dtype=torch.float32, device=index)
         size = L.crx_grads_workspace(n)
         ws = torch.empty(size, dtype=torch.uint8, device=index)
-        st = L.crx_grad_norm(n, _ptrs(tensors), _ext.CBuf("i", [_CODES[t.dtype] for t in tensors]),
-                             _ext.CBuf("q", [t.numel() for t in tensors]), ws.data_ptr(), size, norm.data_ptr(),
-                             _stream(index), err, 512)
+        st = L.crx_grad_norm(n, _ext.ptr_array(ptrs), _ext.CBuf("i", codes), _ext.CBuf("q", numels), ws.data_ptr(), size,
+                             norm.data_ptr(), _stream(index), err, 512)
     if st != _ext.CRX_OK:
         _raise(st, err)
     return norm
@@ -127,18 +139,17 @@ def clip_grads(grads: Mapping[str, torch.Tensor], max_norm: float, *, out: Mappi
     device) takes the place of the gradients' own, for gradients spread over ranks
     (dist.grad_norm_global).  A norm that is not finite is not clipped away: it leaves NaN, as its
     product says.  Tensors that share memory (a tied weight under two names) are refused."""
-    if not max_norm > 0:
+    if not max_norm > 0:   # (NaN too)
         raise ValueError(f"max_norm must be positive, got {max_norm}")
-    tensors, index = _gather("gradients", grads, _CODES, _GRAD_TYPES, None)
+    tensors, ptrs, numels, codes, index = _gather("gradients", grads, _GRADS, _GRAD_TYPES, None)
     if index is None:
         index = _no_tensors()
-    numels = [t.numel() for t in tensors]
-    outs = tensors
+    outs, out_ptrs = tensors, ptrs
     if out is not None:
-        outs = _match("out", out, grads.keys(), numels, _CODES, _GRAD_TYPES, index)
-        for name, g, o in zip(grads, tensors, outs):
-            if g.dtype != o.dtype:
-                raise ValueError(f"{name}: out and the gradient differ in type")
+        outs, out_ptrs, out_codes = _match("out", out, grads.keys(), numels, _GRADS, _GRAD_TYPES, index)
+        if out_codes != codes:
+            name = next(name for name, a, b in zip(grads, codes, out_codes) if a != b)
+            raise ValueError(f"{name}: out and the gradient differ in type")
     if norm is not None:
         _scalar("norm", norm, torch.float32, index)
     L = _ext.load()
@@ -148,8 +159,8 @@ def clip_grads(grads: Mapping[str, torch.Tensor], max_norm: float, *, out: Mappi
         size = 0 if norm is not None else L.crx_grads_workspace(n)
         ws = torch.empty(size, dtype=torch.uint8, device=index) if size else None
         result = norm if norm is not None else torch.empty((), dtype=torch.float32, device=index)
-        st = L.crx_clip_grads(n, _ptrs(tensors), _ptrs(outs), _ext.CBuf("i", [_CODES[t.dtype] for t in tensors]),
-                              _ext.CBuf("q", numels), max_norm, None if norm is None else norm.data_ptr(),
+        st = L.crx_clip_grads(n, _ext.ptr_array(ptrs), _ext.ptr_array(out_ptrs), _ext.CBuf("i", codes), _ext.CBuf("q", numels),
+                              max_norm, None if norm is None else norm.data_ptr(),
                               ws.data_ptr() if size else None, size, result.data_ptr() if norm is None else None,
                               _stream(index), err, 512)
     if st != _ext.CRX_OK:
@@ -171,8 +182,8 @@ def adamw_step(masters: Mapping[str, torch.Tensor], grads: Mapping[str, torch.Te
     is not finite, masters and moments stay as they are (weights get the masters' rounding all the
     same).  `lr` (fp32) and `step` (int64) may be one-element tensors on the device, read when the
     step runs: a captured graph then follows them.  Memory that the step writes may not be shared."""
-    tensors, index = _gather("gradients", grads, _CODES, _GRAD_TYPES, None)
-    names, numels = grads.keys(), [t.numel() for t in tensors]
+    tensors, ptrs, numels, codes, index = _gather("gradients", grads, _GRADS, _GRAD_TYPES, None)
+    names = grads.keys()
     b1, b2 = betas
     if not (0 <= b1 < 1 and 0 <= b2 < 1):
         raise ValueError(f"betas must be in [0, 1), got {betas}")
@@ -186,10 +197,10 @@ def adamw_step(masters: Mapping[str, torch.Tensor], grads: Mapping[str, torch.Te
         raise ValueError(f"step counts from 1, got {step}")
     if not isinstance(lr, torch.Tensor) and not math.isfinite(lr):
         raise ValueError(f"lr must be finite, got {lr}")
-    f32 = (torch.float32,)
-    state = [_match(what, d, names, numels, f32, "float32", index)
-             for what, d in (("masters", masters), ("exp_avg", exp_avg), ("exp_avg_sq", exp_avg_sq))]
-    w = None if weights is None else _match("weights", weights, names, numels, (torch.bfloat16,), "bfloat16", index)
+    (p, p_ptrs, _), (m, m_ptrs, _), (v, v_ptrs, _) = (
+        _match(what, d, names, numels, _F32, "float32", index)
+        for what, d in (("masters", masters), ("exp_avg", exp_avg), ("exp_avg_sq", exp_avg_sq)))
+    w, w_ptrs, _ = ([], None, None) if weights is None else _match("weights", weights, names, numels, _BF16, "bfloat16", index)
     if not tensors:
         return
     for what, t, dtype in (("norm", norm, torch.float32), ("lr", lr, torch.float32), ("step", step, torch.int64)):
@@ -197,20 +208,25 @@ def adamw_step(masters: Mapping[str, torch.Tensor], grads: Mapping[str, torch.Te
             _scalar(what, t, dtype, index)
     lr_p = lr.data_ptr() if isinstance(lr, torch.Tensor) else 0
     step_p = step.data_ptr() if isinstance(step, torch.Tensor) else 0
-    args = struct.pack("5d4qf4x", 0.0 if lr_p else lr, b1, b2, eps, weight_decay, 1 if step_p else int(step), lr_p, step_p,
+    args = _ADAMW.pack(0.0 if lr_p else lr, b1, b2, eps, weight_decay, 1 if step_p else int(step), lr_p, step_p,
                        0 if norm is None else norm.data_ptr(), max_norm or 0.0)
     L = _ext.load()
     err = ctypes.create_string_buffer(512)
     with _on(index):
-        st = L.crx_adamw_step(len(tensors), _ptrs(state[0]), _ptrs(tensors), _ext.CBuf("i", [_CODES[t.dtype] for t in tensors]),
-                              _ptrs(state[1]), _ptrs(state[2]), None if w is None else _ptrs(w), _ext.CBuf("q", numels),
-                              args, _stream(index), err, 512)
+        st = L.crx_adamw_step(len(tensors), _ext.ptr_array(p_ptrs), _ext.ptr_array(ptrs), _ext.CBuf("i", codes),
+                              _ext.ptr_array(m_ptrs), _ext.ptr_array(v_ptrs), None if w_ptrs is None else _ext.ptr_array(w_ptrs),
+                              _ext.CBuf("q", numels), args, _stream(index), err, 512)
     if st != _ext.CRX_OK:
         _raise(st, err)
-    torch.autograd.graph.increment_version(state[0] + state[1] + state[2] + (w or []))
+    torch.autograd.graph.increment_version(p + m + v + w)
 
 
-@dataclass
+_INTS, _MASKS, _NONE = frozenset([torch.int64, torch.int32]), frozenset([torch.bool, torch.float32]), (0, 0, 0)
+_POLICY = struct.Struct("28qd4f4i")    # crx_policy_args
+_ADAMW = struct.Struct("5d4qf4x")      # crx_adamw_args
+
+
+@dataclass(slots=True)
 class PolicyLoss:
     loss: torch.Tensor        # 0-d fp32, differentiable to the logits
     logp: torch.Tensor        # fp32, the tokens' shape: log-probability of each token (0 where it does not count)
@@ -218,17 +234,18 @@ class PolicyLoss:
     clip_frac: torch.Tensor   # 0-d fp32: share of the tokens whose ratio was clipped
 
 
-def _rows(what: str, t, tokens: torch.Tensor, dtypes, types: str, broadcast: bool):
+def _rows(what: str, t, shape, index: int, dtypes, types: str, broadcast: bool):
     """(address, stride over sequences, stride over tokens) of per-token values."""
-    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes:
+    if not isinstance(t, _T) or t.dtype not in dtypes or t.layout is not torch.strided:
         raise ValueError(f"{what}: expected a {types} torch tensor, got {getattr(t, 'dtype', type(t))}")
-    if t.layout != torch.strided or t.dim() != tokens.dim() or any(
-            a != b and not (broadcast and a == 1) for a, b in zip(t.shape, tokens.shape)):
-        raise ValueError(f"{what}: shape {tuple(t.shape)} does not go with tokens {tuple(tokens.shape)}")
-    if t.get_device() != tokens.get_device():
-        raise ValueError("all tensors must be on one device")
-    strides = [0 if t.shape[i] == 1 else t.stride(i) for i in range(t.dim())]
-    return t.data_ptr(), strides[0] if len(strides) == 2 else 0, strides[-1]
+    if t.get_device() != index:
+        raise ValueError(f"{what}: all tensors must be on one device")
+    strides = t.stride()
+    if t.shape != shape:
+        if not broadcast or t.dim() != len(shape) or any(a != b and a != 1 for a, b in zip(t.shape, shape)):
+            raise ValueError(f"{what}: shape {tuple(t.shape)} does not go with tokens {tuple(shape)}")
+        strides = [0 if n == 1 else s for n, s in zip(t.shape, strides)]
+    return (t.data_ptr(), *strides) if len(strides) == 2 else (t.data_ptr(), 0, strides[0])
 
 
 def _grad_like(logits: torch.Tensor) -> torch.Tensor:
@@ -257,25 +274,25 @@ class _Call:
     __slots__ = ("index", "shape", "vocab", "small", "numbers", "keep")
 
     def pack(self, logits, grad, logp, loss, stats, rows) -> bytes:
-        b, t = self.shape
-        two = logits.dim() == 3
-        ls, gs = logits.stride(), logits.stride() if grad is None else grad.stride()
-        return struct.pack("28qd4f4i", b, t, self.vocab, logits.data_ptr(), ls[0] if two else 0, ls[-2],
-                           0 if grad is None else grad.data_ptr(), gs[0] if two else 0, gs[-2], *self.small,
-                           logp.data_ptr(), loss.data_ptr(), stats.data_ptr(), rows.data_ptr(), *self.numbers)
+        ls, g, gs = logits.stride(), 0, (0, 0, 0)
+        if grad is not None:
+            g, gs = grad.data_ptr(), grad.stride()
+        if len(ls) == 2:
+            ls, gs = (0, *ls), (0, *gs)
+        return _POLICY.pack(*self.shape, self.vocab, logits.data_ptr(), ls[0], ls[1], g, gs[0], gs[1], *self.small, logp, loss,
+                            stats, rows, *self.numbers)
 
-    def run(self, logits, grad):
-        L = _ext.load()
-        b, t = self.shape
+    def run(self, logits, want_grad: bool):
+        index, (b, t) = self.index, self.shape
         err = ctypes.create_string_buffer(512)
-        with _on(self.index):
-            if grad:
-                grad = _grad_like(logits)
-            loss = torch.empty((), dtype=torch.float32, device=self.index)
-            stats = torch.empty(2, dtype=torch.float32, device=self.index)
-            logp = torch.empty(self.keep[0].shape, dtype=torch.float32, device=self.index)
-            rows = torch.empty(L.crx_policy_workspace(b, t), dtype=torch.uint8, device=self.index)
-            st = L.crx_policy_loss(self.pack(logits, grad, logp, loss, stats, rows), _stream(self.index), err, 512)
+        with _on(index):
+            grad = _grad_like(logits) if want_grad else None
+            loss = torch.empty((), dtype=torch.float32, device=logits.device)
+            logp = torch.empty(self.keep[0].shape, dtype=torch.float32, device=logits.device)
+            stats = torch.empty(2, dtype=torch.float32, device=logits.device)
+            rows = torch.empty(_ext.load().crx_policy_workspace(b, t), dtype=torch.uint8, device=logits.device)
+            st = _ext.load().crx_policy_loss(
+                self.pack(logits, grad, logp.data_ptr(), loss.data_ptr(), stats.data_ptr(), rows.data_ptr()), _stream(index), err, 512)
         if st != _ext.CRX_OK:
             _raise(st, err)
         return loss, stats, logp, rows, grad
@@ -309,7 +326,8 @@ class _PolicyLossFn(torch.autograd.Function):
             unless_one = grad is not None
             if grad is None:
                 grad = _grad_like(logits)
-            st = _ext.load().crx_policy_backward(call.pack(logits, grad, ctx.rows, ctx.rows, ctx.rows, ctx.rows), scale.data_ptr(), unless_one,
+            rows = ctx.rows.data_ptr()   # (in the places of results that the backward pass does not touch, too)
+            st = _ext.load().crx_policy_backward(call.pack(logits, grad, rows, rows, rows, rows), scale.data_ptr(), unless_one,
                                                  _stream(call.index), err, 512)
         if st != _ext.CRX_OK:
             _raise(st, err)
@@ -338,37 +356,32 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, advantages: torch.Te
 
     Where the logits require a gradient it is computed in this same call (they are read once), for
     loss.backward() as it stands; a loss that is scaled first is right too, and costs a second pass."""
-    if not isinstance(logits, torch.Tensor) or logits.dtype not in _CODES:
+    if not isinstance(logits, _T) or logits.dtype not in _CODES or logits.layout is not torch.strided:
         raise ValueError(f"logits: expected a {_GRAD_TYPES} torch tensor, got {getattr(logits, 'dtype', type(logits))}")
-    if not isinstance(tokens, torch.Tensor) or tokens.dtype not in (torch.int64, torch.int32):
-        raise ValueError(f"tokens: expected an int64 or int32 torch tensor, got {getattr(tokens, 'dtype', type(tokens))}")
-    if logits.layout != torch.strided or tokens.dim() not in (1, 2) or logits.shape[:-1] != tokens.shape or logits.dim() < 2 \
-            or logits.shape[-1] < 1:
-        raise ValueError(f"logits {tuple(logits.shape)} do not go with tokens {tuple(tokens.shape)}: "
+    if not isinstance(tokens, _T):
+        raise ValueError(f"tokens: expected an int64 or int32 torch tensor, got {type(tokens)}")
+    size, shape = logits.shape, tokens.shape
+    if len(shape) not in (1, 2) or size[:-1] != shape or len(size) < 2 or size[-1] < 1:
+        raise ValueError(f"logits {tuple(size)} do not go with tokens {tuple(shape)}: "
                          "expected [T, V] and [T], or [B, T, V] and [B, T]")
-    if logits.shape[-1] > 1 and logits.stride(-1) != 1:
+    if size[-1] > 1 and logits.stride(-1) != 1:
         raise ValueError("logits: the vocabulary must be contiguous")
     if not logits.is_cuda:
         raise ValueError("logits: expected a CUDA tensor")
-    f32 = (torch.float32,)
     call = _Call()
-    call.index = logits.get_device()
-    two = tokens.dim() == 2
-    call.shape = tuple(tokens.shape) if two else (1, tokens.shape[0])
-    call.vocab = logits.shape[-1]
-    if tokens.get_device() != call.index:
-        raise ValueError("all tensors must be on one device")
-    none = (0, 0, 0)
+    index = call.index = logits.get_device()
+    call.shape = shape if len(shape) == 2 else (1, shape[0])
+    call.vocab = size[-1]
     call.small = (
-        *_rows("tokens", tokens, tokens, (torch.int64, torch.int32), "int64 or int32", False),
-        *_rows("advantages", advantages, tokens, f32, "float32", True),
-        *(none if old_logp is None else _rows("old_logp", old_logp, tokens, f32, "float32", False)),
-        *(none if ref_logp is None else _rows("ref_logp", ref_logp, tokens, f32, "float32", False)),
-        *(none if mask is None else _rows("mask", mask, tokens, (torch.bool, torch.float32), "bool or float32", True)))
+        *_rows("tokens", tokens, shape, index, _INTS, "int64 or int32", False),
+        *_rows("advantages", advantages, shape, index, _F32, "float32", True),
+        *(_NONE if old_logp is None else _rows("old_logp", old_logp, shape, index, _F32, "float32", False)),
+        *(_NONE if ref_logp is None else _rows("ref_logp", ref_logp, shape, index, _F32, "float32", False)),
+        *(_NONE if mask is None else _rows("mask", mask, shape, index, _MASKS, "bool or float32", True)))
     lo, hi = clip
     if not (lo >= 0 and hi >= 0):
         raise ValueError(f"clip bounds must not be negative, got {clip}")
-    if not (temperature > 0 and math.isfinite(temperature)):
+    if not 0 < temperature < math.inf:
         raise ValueError(f"temperature must be positive and finite, got {temperature}")
     if not math.isfinite(kl_coef):
         raise ValueError(f"kl_coef must be finite, got {kl_coef}")
@@ -381,6 +394,6 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, advantages: torch.Te
     call.keep = (tokens, advantages, old_logp, ref_logp, mask)
     if logits.requires_grad and torch.is_grad_enabled():
         return PolicyLoss(*_PolicyLossFn.apply(logits, call))
-    loss, stats, logp, _, _ = call.run(logits, None)
+    loss, stats, logp, _, _ = call.run(logits, False)
     kl, clip_frac = stats.unbind(0)
     return PolicyLoss(loss, logp, kl, clip_frac)
