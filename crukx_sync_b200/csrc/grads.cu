@@ -1,12 +1,11 @@
 // Whole-model passes of a trainer over its gradients and its fp32 masters, between the backward
 // pass and the encode of the update (no reference counterpart: the reference starts at the two
-// weight dicts).  n tensors of any sizes per call, every tensor cut into tiles, tiles dealt to a
-// persistent grid in contiguous ranges:
+// weight dicts).  n tensors of any sizes per call, every tensor cut into tiles:
 //
 //   k_grad_sumsq   sum of squares of every gradient: one partial (double) per CTA
 //   k_grad_norm    one CTA: the partials summed in a fixed order, and the square root
-//   k_grad_clip    every CTA sums the partials itself (same order, so the same coefficient
-//                  everywhere), then out = min(1, max_norm / (norm + 1e-6)) * grad over its tiles
+//   k_grad_clip    out = min(1, max_norm / (norm + 1e-6)) * grad; where there are few partials every
+//                  CTA sums them itself (same order, so the same coefficient everywhere)
 //   k_adamw        AdamW on fp32 masters and moments with that coefficient folded in, and the
 //                  bf16 weights written beside them
 //
@@ -33,7 +32,16 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kTile = 8192;            // gradient elements per tile of the norm and the clip
 constexpr int kStepTile = kThreads * 8;   // parameters per tile of the step: 8 per thread
-constexpr int kMaxGrid = 148 * 8;      // most CTAs of one launch, so most partials of it
+// CTAs of one launch of the norm, at most, and so its partials.  Each takes a contiguous range of
+// tiles (of 330 tensors and 2 GB: 343 us; every grid-th tile, which passes more tensors: 428).  Four times
+// as many CTAs as fit the GPU at once: their ends spread, so the last wave is short (1.86 GB of bf16:
+// 362 us with 8 per SM, 325 with 32 and with 64).
+constexpr int kMaxGrid = 148 * 32;
+// The clip and the step have one CTA per tile.  A CTA whose stores are still on their way holds
+// nobody up, and the hardware deals the tiles out as SMs come free: 0.93e9 parameters took 4.37 ms
+// with 16 CTAs per SM walking a range of tiles each, 4.13 with 64, 3.81 with one CTA per tile; the
+// clip of 1.86 GB 0.59 and 0.54.
+constexpr int kClipPartials = 1024;    // up to here each CTA of the clip sums the partials itself
 
 struct GradEntry {
     const void* g;
@@ -153,7 +161,7 @@ __global__ void __launch_bounds__(kThreads) k_grad_sumsq(const __grid_constant__
     const uint32_t lo = uint32_t(uint64_t(t.tiles) * blockIdx.x / gridDim.x);
     const uint32_t hi = uint32_t(uint64_t(t.tiles) * (blockIdx.x + 1) / gridDim.x);
     double acc = 0;
-    int i = lo < hi ? tensor_of(t, lo) : 0;
+    int i = tensor_of(t, lo);
     for (uint32_t s = lo; s < hi; ++s) {
         while (i + 1 < t.n && t.e[i + 1].tile <= s) ++i;
         const int64_t k = s - t.e[i].tile;
@@ -219,30 +227,23 @@ __device__ __forceinline__ void tile_scale(const T* g, T* out, int64_t numel, in
     for (int64_t i = int64_t(nv) * N + tid; i < n; i += kThreads) o[i] = from_f<T>(c * to_f(p[i]));
 }
 
-// CTAs walk their tiles from the last to the first: the pass before read them in the other order,
-// so the first ones taken here are what L2 still holds.
+// The tiles from the last to the first: the norm took them the other way, so the first ones here are
+// what L2 still holds.
 template <class Tab>
 __global__ void __launch_bounds__(kThreads) k_grad_clip(const __grid_constant__ Tab t, const double* __restrict__ partials,
                                                         int n_partials, const float* __restrict__ norm_in, float max_norm,
                                                         float* __restrict__ norm_out) {
     __shared__ double red[kThreads / 32];
-    const float norm = norm_in ? *norm_in : float(sqrt(sum_partials(partials, n_partials, red)));
+    const float norm = n_partials ? float(sqrt(sum_partials(partials, n_partials, red))) : *norm_in;
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
     const float c = clip_coef(norm, max_norm);
-    const uint32_t lo = uint32_t(uint64_t(t.tiles) * blockIdx.x / gridDim.x);
-    const uint32_t hi = uint32_t(uint64_t(t.tiles) * (blockIdx.x + 1) / gridDim.x);
-    int i = lo < hi ? tensor_of(t, hi - 1) : 0;
-    for (uint32_t s = hi; s-- > lo;) {
-        while (t.e[i].tile > s) --i;
-        if (c == 1.f && t.e[i].out == t.e[i].g) continue;   // in place and nothing to scale
-        const int64_t k = s - t.e[i].tile;
-        if (t.e[i].dtype == CRX_FP32)
-            tile_scale(static_cast<const float*>(t.e[i].g), static_cast<float*>(t.e[i].out), t.e[i].numel, k, c);
-        else if (t.e[i].dtype == CRX_BF16)
-            tile_scale(static_cast<const __nv_bfloat16*>(t.e[i].g), static_cast<__nv_bfloat16*>(t.e[i].out), t.e[i].numel, k, c);
-        else
-            tile_scale(static_cast<const __half*>(t.e[i].g), static_cast<__half*>(t.e[i].out), t.e[i].numel, k, c);
-    }
+    const uint32_t s = t.tiles - 1 - blockIdx.x;
+    const GradEntry& e = t.e[tensor_of(t, s)];
+    if (c == 1.f && e.out == e.g) return;   // in place and nothing to scale
+    const int64_t k = s - e.tile;
+    if (e.dtype == CRX_FP32) tile_scale(static_cast<const float*>(e.g), static_cast<float*>(e.out), e.numel, k, c);
+    else if (e.dtype == CRX_BF16) tile_scale(static_cast<const __nv_bfloat16*>(e.g), static_cast<__nv_bfloat16*>(e.out), e.numel, k, c);
+    else tile_scale(static_cast<const __half*>(e.g), static_cast<__half*>(e.out), e.numel, k, c);
 }
 
 struct StepHyper {
@@ -261,12 +262,25 @@ struct StepRates {
     bool skip;   // the norm is not finite: masters and moments stay as they are
 };
 
+// Root and reciprocal to 1 ulp each: the exact ones took the step of 0.93e9 parameters from 3.81 to
+// 4.87 ms, for two roundings that are 2^-24 of an update that is itself a small part of the master.
+__device__ __forceinline__ float sqrt_fast(float x) {
+    float y;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+    float y;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 __device__ __forceinline__ void adamw_one(const StepRates& r, float g, float& p, float& m, float& v) {
     g *= r.c;
     m = fmaf(r.b1, m, r.a1 * g);
     v = fmaf(r.b2, v, r.a2 * g * g);
-    const float den = sqrtf(v * r.inv_bias2) + r.eps;
-    p -= fmaf(r.decay, p, (r.rate * m) / den);   // both terms first: p is rounded once
+    const float den = sqrt_fast(v * r.inv_bias2) + r.eps;
+    p -= fmaf(r.decay, p, (r.rate * m) * rcp_fast(den));   // both terms first: p is rounded once
 }
 
 template <class T>
@@ -349,16 +363,11 @@ __global__ void __launch_bounds__(kThreads) k_adamw(const __grid_constant__ Tab 
     r.rate = lr / bias1;
     r.inv_bias2 = 1.f / bias2;
     r.eps = h.eps;
-    const uint32_t lo = uint32_t(uint64_t(t.tiles) * blockIdx.x / gridDim.x);
-    const uint32_t hi = uint32_t(uint64_t(t.tiles) * (blockIdx.x + 1) / gridDim.x);
-    int i = lo < hi ? tensor_of(t, lo) : 0;
-    for (uint32_t s = lo; s < hi; ++s) {
-        while (i + 1 < t.n && t.e[i + 1].tile <= s) ++i;
-        const int64_t k = s - t.e[i].tile;
-        if (t.e[i].dtype == CRX_FP32) tile_step<float>(t.e[i], r, k);
-        else if (t.e[i].dtype == CRX_BF16) tile_step<__nv_bfloat16>(t.e[i], r, k);
-        else tile_step<__half>(t.e[i], r, k);
-    }
+    const StepEntry& e = t.e[tensor_of(t, blockIdx.x)];
+    const int64_t k = blockIdx.x - e.tile;
+    if (e.dtype == CRX_FP32) tile_step<float>(e, r, k);
+    else if (e.dtype == CRX_BF16) tile_step<__nv_bfloat16>(e, r, k);
+    else tile_step<__half>(e, r, k);
 }
 
 // ------------------------------------------------------------------ host
@@ -411,8 +420,6 @@ int check_common(const char* who, int32_t n, const void* const* grads, const int
     return CRX_OK;
 }
 
-int grid_for(uint32_t tiles, int per_sm) { return int(std::min<uint32_t>(tiles, uint32_t(148 * per_sm))); }
-
 uint32_t grad_tiles(const void* g, int64_t numel, int dtype) {
     const int head = dtype == CRX_FP32 ? head_of<float>(g) : head_of<__half>(g);
     const int64_t body = std::max<int64_t>(0, numel - head);
@@ -431,7 +438,7 @@ cudaError_t each_table(int32_t n, const int64_t* numel, int32_t* at, Fill fill, 
         E& e = t.e[t.n];
         e.tile = t.tiles;
         const uint32_t tiles = fill(e, i);
-        if (uint64_t(t.tiles) + tiles > 0xffffffffull) break;   // the rest goes into the next launch
+        if (uint64_t(t.tiles) + tiles > 0x7fffffffull) break;   // a grid's most: the rest goes into the next launch
         t.tiles += tiles;
         ++t.n;
     }
@@ -467,7 +474,7 @@ cudaError_t launch_sumsq(int32_t n, const void* const* grads, const int32_t* dty
             return grad_tiles(grads[i], numel[i], dtypes[i]);
         },
         [&](const auto& t) {
-            const int grid = grid_for(t.tiles, 8);
+            const int grid = int(std::min<uint32_t>(t.tiles, kMaxGrid));
             k_grad_sumsq<<<grid, kThreads, 0, st>>>(t, partials + *count);
             *count += grid;
             return cudaGetLastError();
@@ -530,7 +537,14 @@ int crx_clip_grads(int32_t n, const void* const* grads, void* const* out, const 
         double* partials = static_cast<double*>(workspace);
         int count = 0;
         cudaError_t e = norm_in ? cudaSuccess : launch_sumsq(n, grads, dtypes, numel, partials, &count, st);
-        float* write_norm = norm_out;   // by the first launch
+        float* write_norm = norm_out;   // by the first launch that knows it
+        if (e == cudaSuccess && count > kClipPartials) {
+            k_grad_norm<<<1, kThreads, 0, st>>>(partials, count, norm_out);
+            e = cudaGetLastError();
+            norm_in = norm_out;
+            write_norm = nullptr;
+            count = 0;
+        }
         if (e == cudaSuccess)
             e = all_tables<GradEntry, kGradLarge>(
                 n, numel,
@@ -542,7 +556,7 @@ int crx_clip_grads(int32_t n, const void* const* grads, void* const* out, const 
                     return grad_tiles(grads[i], numel[i], dtypes[i]);
                 },
                 [&](const auto& t) {
-                    k_grad_clip<<<grid_for(t.tiles, 8), kThreads, 0, st>>>(t, partials, count, norm_in, max_norm, write_norm);
+                    k_grad_clip<<<t.tiles, kThreads, 0, st>>>(t, partials, count, norm_in, max_norm, write_norm);
                     write_norm = nullptr;
                     return cudaGetLastError();
                 });
@@ -622,7 +636,7 @@ int crx_adamw_step(int32_t n, float* const* master, const void* const* grads, co
                 return uint32_t(std::max<int64_t>(1, (body + kStepTile - 1) / kStepTile));
             },
             [&](const auto& t) {
-                k_adamw<<<grid_for(t.tiles, 4), kThreads, 0, st>>>(t, h);
+                k_adamw<<<t.tiles, kThreads, 0, st>>>(t, h);
                 return cudaGetLastError();
             });
         return e == cudaSuccess ? CRX_OK : cuda_fail(err, errlen, "crx_adamw_step", e);
