@@ -13,6 +13,7 @@ namespace crx {
 template <class T> struct Vec;   // 16 bytes of T
 template <> struct Vec<float> {
     static constexpr int N = 4;
+    static __device__ __forceinline__ uint4 lowest() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }   // -inf
     static __device__ __forceinline__ void get(const uint4& q, float* x) {
         x[0] = __uint_as_float(q.x); x[1] = __uint_as_float(q.y); x[2] = __uint_as_float(q.z); x[3] = __uint_as_float(q.w);
     }
@@ -22,6 +23,7 @@ template <> struct Vec<float> {
 };
 template <> struct Vec<__nv_bfloat16> {
     static constexpr int N = 8;
+    static __device__ __forceinline__ uint4 lowest() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
     static __device__ __forceinline__ void get(const uint4& q, float* x) {
         const uint32_t u[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
@@ -42,6 +44,7 @@ template <> struct Vec<__nv_bfloat16> {
 };
 template <> struct Vec<__half> {
     static constexpr int N = 8;
+    static __device__ __forceinline__ uint4 lowest() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
     static __device__ __forceinline__ void get(const uint4& q, float* x) {
         const uint32_t u[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll

@@ -8,16 +8,19 @@
 // u depends on the row's own logp alone (D is known before), so the gradient is written in the
 // same visit to the row: the logits are read from HBM once and written once.
 //
-//   k_policy_denom   one CTA: 1 / sum of the mask (only where the caller gives no denominator)
-//   k_policy_rows    a cluster of CTAs per row, rows dealt to the clusters of a persistent grid;
-//                    each CTA has a slice of the row; the (M, s) of the slices meet through
-//                    distributed shared memory; then the gradient, from the slice again (L2)
-//   k_policy_sums    one CTA: the rows' terms summed in a fixed order, in double
+//   k_policy_plan    one CTA, where there is a mask: 1 / its sum, and the rows in the order in which
+//                    they are taken: those that count, then the others (whose gradient is 0)
+//   k_policy_rows    a warp, a CTA or a cluster of CTAs per row, rows dealt to a persistent grid.
+//                    Every warp streams its part of the rows through a ring of its own in shared
+//                    memory, filled by bulk copies that run ahead into the next rows while this one
+//                    is reduced; a row that fits its ring is turned into the gradient from there
+//   k_policy_sums    one CTA: the terms of the rows summed in a fixed order, in double
 //   k_policy_again   the gradient once more, scaled, from the rows' saved (u, R, s)
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdio>
 #include <exception>
@@ -32,10 +35,17 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kRowThreads = 512;
+constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32;
 constexpr int kMaxCluster = 8;
+constexpr int kRowCtas = 2;            // per SM
+constexpr int kSlots = 6;              // of a warp's ring
+constexpr int kChunk = 128;            // 16-byte vectors of a slot: four per lane
+constexpr int kRowGrid = 148 * kRowCtas;       // CTAs of the persistent grid
+constexpr int kMaxUnits = kRowGrid * kRowWarps;
+constexpr size_t kRingBytes = size_t(kRowWarps) * kSlots * kChunk * 16;
 constexpr float kFar = 3e38f;
+constexpr int kMaxDevices = 64;
 
 // 2^x to about 2 ulp; results below 2^-126 become 0, which neither a sum of at least 1 nor a
 // gradient in any of the types can tell from them.
@@ -54,14 +64,19 @@ __device__ __forceinline__ float weight(const crx_policy_args& a, int64_t b, int
     return static_cast<const uint8_t*>(a.mask.p)[at(a.mask, b, t)] ? 1.f : 0.f;
 }
 
-// Layout of args.rows: 1 / denominator (double, 16 bytes), a float4 per row, then the sums of the
-// three terms over each cluster's rows (double).  A row's float4 is (u, R, s, 0), or (u, M, s, 1)
-// for a far row (below).
-__host__ __device__ __forceinline__ double* inv_denom_of(const crx_policy_args& a) { return reinterpret_cast<double*>(a.rows); }
+// Layout of args.rows: the plan's 1 / denominator and number of rows that count, a float4 per row,
+// the sums of the three terms over each unit's rows (double), the plan's order of the rows.  A row's
+// float4 is (u, R, s, 0), or (u, M, s, 1) for a far row (below).
+struct Plan {
+    double inv_denom;
+    int64_t counted;
+};
+__host__ __device__ __forceinline__ Plan* plan_of(const crx_policy_args& a) { return reinterpret_cast<Plan*>(a.rows); }
 __device__ __forceinline__ float4* saved_of(const crx_policy_args& a) { return reinterpret_cast<float4*>(a.rows) + 1; }
-__host__ __device__ __forceinline__ double* partials_of(const crx_policy_args& a) {
+__device__ __forceinline__ double* partials_of(const crx_policy_args& a) {
     return reinterpret_cast<double*>(a.rows + 4 + 4 * a.batch * a.steps);
 }
+__device__ __forceinline__ int32_t* order_of(const crx_policy_args& a) { return reinterpret_cast<int32_t*>(partials_of(a) + 3 * kMaxUnits); }
 
 // The largest of N packed values (NaNs lose; they show in the sum).
 template <class T> __device__ __forceinline__ float vec_max(const uint4* q, int n);
@@ -114,13 +129,6 @@ struct Running {
             r = r2;
         }
     }
-    __device__ __forceinline__ void join(float m2, float s2, float c) {
-        const float r2 = fmaxf(m2 * c, -kFar);
-        const float big = fmaxf(r, r2);
-        s = s * exp2_fast(r - big) + s2 * exp2_fast(r2 - big);
-        r = big;
-        m = fmaxf(m, m2);
-    }
 };
 
 template <class T, int U>
@@ -140,21 +148,21 @@ __device__ __forceinline__ void add_vecs(const uint4* q, Running& run, float c) 
     run.s += a + b;
 }
 
-// A CTA's slice of a row: 16-byte vectors [lo, hi) of the part after the row's first 16-byte
-// boundary; the first CTA also has the elements before it and the row's last ones.
+// A CTA's (or warp's) slice of a row: 16-byte vectors [lo, hi) of the part after the row's first
+// 16-byte boundary; the first CTA also has the elements before it and the row's last ones.
 struct Slice {
     int head, tail;   // elements before the boundary, and after the last whole vector (first CTA)
-    int64_t body;     // element of the first whole vector
-    int64_t tail_at;  // element where the tail begins
-    int64_t lo, hi;
+    int body;         // element of the first whole vector
+    int tail_at;      // element where the tail begins
+    int lo, hi;
 };
 template <class T>
 __device__ __forceinline__ Slice slice_of(const T* z, int64_t V, int rank, int C) {
     Slice s;
     const int head = int(tmin<int64_t>(head_of<T>(z), V));
-    const int64_t nv = (V - head) / Vec<T>::N;
-    s.lo = nv * rank / C;
-    s.hi = nv * (rank + 1) / C;
+    const int nv = int((V - head) / Vec<T>::N);
+    s.lo = int(int64_t(nv) * rank / C);
+    s.hi = int(int64_t(nv) * (rank + 1) / C);
     s.head = rank ? 0 : head;
     s.body = head;
     s.tail_at = head + nv * Vec<T>::N;
@@ -167,34 +175,61 @@ struct Shared {
     float2 part[2][kMaxCluster];   // (M, s) of every CTA of the cluster, double-buffered over rows
 };
 
-// (M, s) of the whole row from every thread's; the same bits in every thread of the cluster.
-__device__ __forceinline__ Running row_total(Running run, Shared& sh, int parity, int rank, int C, float c) {
-    for (int o = 16; o; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, run.m, o), s2 = __shfl_xor_sync(0xffffffffu, run.s, o);
-        run.join(m2, s2, c);
+// The largest of a warp's values: as integers of the same order, one instruction for the warp.
+__device__ __forceinline__ float warp_max(float x) {
+    const int i = __float_as_int(x);
+    const int k = __reduce_max_sync(0xffffffffu, i ^ ((i >> 31) & 0x7fffffff));
+    return __int_as_float(k ^ ((k >> 31) & 0x7fffffff));
+}
+
+// (M, s) over the lanes of a warp: the maximum first, then one rescaling per lane and a sum.
+__device__ __forceinline__ Running warp_total(Running run, float c) {
+    const float m = warp_max(run.m);
+    Running all;
+    all.m = m;
+    all.r = fmaxf(m * c, -kFar);
+    float s = run.s * exp2_fast(fmaxf(run.m * c, -kFar) - all.r);
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    all.s = s;
+    return all;
+}
+__device__ __forceinline__ Running lane_entry(const float2* e, int n) {
+    const int lane = threadIdx.x & 31;
+    Running r;
+    if (lane < n) {
+        const float2 v = e[lane];
+        r.m = v.x;
+        r.s = v.y;
     }
+    return r;
+}
+
+// (M, s) of the whole row from every thread's; the same bits in every thread of the cluster.
+template <bool WARP>
+__device__ __forceinline__ Running row_total(Running run, Shared& sh, int parity, int rank, int C, float c) {
+    run = warp_total(run, c);
+    if (WARP) return run;
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (lane == 0) sh.warp[w] = make_float2(run.m, run.s);
     __syncthreads();
-    Running all;
     if (C == 1) {
-        for (int k = 0; k < kRowWarps; ++k) all.join(sh.warp[k].x, sh.warp[k].y, c);
+        run = warp_total(lane_entry(sh.warp, kRowWarps), c);
         __syncthreads();   // sh.warp is written again by the next row
-        return all;
+        return run;
     }
     cg::cluster_group cl = cg::this_cluster();
     if (w == 0) {
-        for (int k = 0; k < kRowWarps; ++k) all.join(sh.warp[k].x, sh.warp[k].y, c);
-        if (lane < C) *cl.map_shared_rank(&sh.part[parity][rank], lane) = make_float2(all.m, all.s);
+        run = warp_total(lane_entry(sh.warp, kRowWarps), c);
+        if (lane < C) *cl.map_shared_rank(&sh.part[parity][rank], lane) = make_float2(run.m, run.s);
     }
     cl.sync();
-    all = Running();
-    for (int k = 0; k < C; ++k) all.join(sh.part[parity][k].x, sh.part[parity][k].y, c);
-    return all;
+    return warp_total(lane_entry(sh.part[parity], C), c);
 }
 
-__device__ __forceinline__ float block_total(float v, Shared& sh) {
+template <bool WARP>
+__device__ __forceinline__ float unit_total(float v, Shared& sh) {
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (WARP) return v;
     __syncthreads();
     if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5].y = v;
     __syncthreads();
@@ -207,155 +242,95 @@ __device__ __forceinline__ float block_total(float v, Shared& sh) {
 // The sum of a far row: one whose largest logit M is so large in magnitude that M c does not fit
 // fp32 (every logit the type's lowest value, say).  (z - M) c takes the place of z c - R, and each
 // CTA of the cluster goes over the whole row.
-template <class T>
+template <class T, bool WARP>
 __device__ __noinline__ float far_sum(const T* z, int64_t V, float M, float c, Shared& sh) {
     float s = 0.f;
-    for (int64_t j = threadIdx.x; j < V; j += kRowThreads) s += exp2_fast((to_f(z[j]) - M) * c);
-    return block_total(s, sh);
+    for (int64_t j = WARP ? threadIdx.x & 31 : threadIdx.x; j < V; j += WARP ? 32 : kRowThreads) s += exp2_fast((to_f(z[j]) - M) * c);
+    return unit_total<WARP>(s, sh);
 }
 
-// The gradient over one CTA's slice, u 1[j = a] - k 2^(z_j c - R) with k = u / s.  u = 0 (a clipped
-// token without a KL term, a token that does not count) writes zeros and reads nothing.
+// What turns a row's logits into its gradient, u 1[j = a] - k 2^(z_j c - R) with k = u / s.  u = 0 (a
+// clipped token without a KL term, a token that does not count) gives zeros whatever the logits.
 template <class T>
-__device__ __forceinline__ void write_grad(const T* z, T* g, const Slice& sl, int64_t V, int64_t token, float u, float R, float s,
-                                           float c, bool far) {
-    constexpr int N = Vec<T>::N;
-    const int tid = threadIdx.x;
-    const float k = u == 0.f ? 0.f : u / s;
-    const auto one = [&](int64_t j) {
+struct GradOf {
+    static constexpr int N = Vec<T>::N;
+    const T* z;
+    T* g;
+    int64_t token;
+    float u, k, R, c;
+    bool far, wide;   // wide: gradient rows start at the same place between 16-byte boundaries as the logits'
+    int token_vec;
+
+    __device__ __forceinline__ GradOf(const T* z, T* g, const Slice& sl, int64_t token, float u, float R, float s, float c, bool far)
+        : z(z), g(g), token(token), u(u), k(u == 0.f ? 0.f : u / s), R(R), c(c), far(far) {
+        wide = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
+        token_vec = token >= sl.body ? int((token - sl.body) / N) : -1;
+    }
+    __device__ __forceinline__ void one(int64_t j, float f) const {
         float x = 0.f;
         if (u != 0.f) {
-            const float f = to_f(z[j]);
             x = -k * exp2_fast(far ? (f - R) * c : fmaf(f, c, -R));
             if (j == token) x += u;
         }
         g[j] = from_f<T>(x);
-    };
-    if (tid < sl.head) one(tid);
-    if (tid < sl.tail) one(sl.tail_at + tid);
-    const int64_t body = sl.body;
-    const bool wide = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
-    if (!wide || far) {
-        for (int64_t j = body + sl.lo * N + tid; j < body + sl.hi * N; j += kRowThreads) one(j);
-        return;
     }
-    const uint4* zv = reinterpret_cast<const uint4*>(z + body);
-    uint4* gv = reinterpret_cast<uint4*>(g + body);
-    if (u == 0.f) {
-        for (int64_t i = sl.lo + tid; i < sl.hi; i += kRowThreads) gv[i] = make_uint4(0, 0, 0, 0);
-        return;
-    }
-    const int64_t token_vec = token >= body ? (token - body) / N : -1;
-    const auto vec = [&](int64_t i, const uint4& q) {
+    __device__ __forceinline__ void one(int64_t j) const { one(j, u == 0.f ? 0.f : to_f(z[j])); }
+    // vector i of the body, its logits in q
+    __device__ __forceinline__ void vec(int body, int i, const uint4& q) const {
         float x[N];
-        Vec<T>::get(q, x);
+        if (u == 0.f) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) x[e] = -k * exp2_fast(fmaf(x[e], c, -R));
-        if (i == token_vec) {
+            for (int e = 0; e < N; ++e) x[e] = 0.f;
+        } else {
+            Vec<T>::get(q, x);
+            if (far || !wide) {
 #pragma unroll
-            for (int e = 0; e < N; ++e)
-                if (body + i * N + e == token) x[e] += u;
-        }
-        gv[i] = Vec<T>::put(x);
-    };
-    constexpr int U = 4;
-    int64_t i = sl.lo + tid;
-    for (; i + (U - 1) * kRowThreads < sl.hi; i += U * kRowThreads) {
-        uint4 q[U];
-#pragma unroll
-        for (int v = 0; v < U; ++v) q[v] = zv[i + v * kRowThreads];
-#pragma unroll
-        for (int v = 0; v < U; ++v) vec(i + v * kRowThreads, q[v]);
-    }
-    for (; i < sl.hi; i += kRowThreads) vec(i, zv[i]);
-}
-
-template <class T, bool GRAD>
-__global__ void __launch_bounds__(kRowThreads) k_policy_rows(const __grid_constant__ crx_policy_args a, double inv_denom, int C) {
-    __shared__ Shared sh;
-    const int tid = threadIdx.x, rank = int(blockIdx.x) % C;
-    const int64_t n = a.batch * a.steps, V = a.vocab, clusters = gridDim.x / C;
-    const float c = float(1.4426950408889634 / double(a.temperature));
-    const double inv_d = inv_denom < 0 ? *inv_denom_of(a) : inv_denom;
-    double loss = 0, kl = 0, cut = 0;
-    int parity = 0;
-    if (C > 1) cg::this_cluster().sync();   // every CTA runs before another writes to its shared memory
-    for (int64_t row = blockIdx.x / C; row < n; row += clusters) {
-        const int64_t b = row / a.steps, t = row - b * a.steps;
-        const float w = weight(a, b, t);
-        const T* z = static_cast<const T*>(a.logits.p) + at(a.logits, b, t);
-        T* g = GRAD ? static_cast<T*>(const_cast<void*>(a.grad.p)) + at(a.grad, b, t) : nullptr;
-        const Slice sl = slice_of<T>(z, V, rank, C);
-        if (w == 0.f) {
-            if (GRAD) write_grad<T>(z, g, sl, V, -1, 0.f, 0.f, 1.f, c, false);
-            if (rank == 0 && tid == 0) {
-                a.logp[row] = 0.f;
-                saved_of(a)[row] = make_float4(0.f, 0.f, 1.f, 0.f);
+                for (int e = 0; e < N; ++e) one(body + int64_t(i) * N + e, x[e]);
+                return;
             }
-            continue;
-        }
-        const int64_t token = a.tokens64 ? static_cast<const int64_t*>(a.tokens.p)[at(a.tokens, b, t)]
-                                         : static_cast<const int32_t*>(a.tokens.p)[at(a.tokens, b, t)];
-        const float za = token >= 0 && token < V ? to_f(z[token]) : NAN;
-        const float A = value(a.advantages, b, t);
-        const float old = a.old_logp.p ? value(a.old_logp, b, t) : 0.f;
-        const float ref = a.ref_logp.p ? value(a.ref_logp, b, t) : 0.f;
-
-        Running run;
-        {
-            const auto one = [&](int64_t j) {
-                const float x = to_f(z[j]);
-                run.raise(x, c);
-                run.s += exp2_fast(fmaf(x, c, -run.r));
-            };
-            if (tid < sl.head) one(tid);
-            if (tid < sl.tail) one(sl.tail_at + tid);
-            const uint4* zv = reinterpret_cast<const uint4*>(z + sl.body);
-            constexpr int U = 4;
-            int64_t i = sl.lo + tid;
-            for (; i + (U - 1) * kRowThreads < sl.hi; i += U * kRowThreads) {
-                uint4 q[U];
 #pragma unroll
-                for (int v = 0; v < U; ++v) q[v] = zv[i + v * kRowThreads];
-                add_vecs<T, U>(q, run, c);
-            }
-            for (; i < sl.hi; i += kRowThreads) {
-                const uint4 q = zv[i];
-                add_vecs<T, 1>(&q, run, c);
+            for (int e = 0; e < N; ++e) x[e] = -k * exp2_fast(fmaf(x[e], c, -R));
+            if (i == token_vec) {
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (body + int64_t(i) * N + e == token) x[e] += u;
             }
         }
-        run = row_total(run, sh, parity, rank, C, c);
-        parity ^= 1;
-        const bool far = fabsf(run.m) <= 3.402823466e38f && !(fabsf(run.m * c) < kFar);
-        const float s = far ? far_sum<T>(z, V, run.m, c, sh) : run.s;
-        const float R = far ? run.m : run.r;
-        const float logp = ((far ? (za - R) * c : fmaf(za, c, -R)) - log2f(s)) * 0.6931471805599453f;
+        T* o = g + body + int64_t(i) * N;
+        if (wide) *reinterpret_cast<uint4*>(o) = Vec<T>::put(x);
+        else
+            for (int e = 0; e < N; ++e) o[e] = from_f<T>(x[e]);
+    }
+    // a slice from global memory, by `threads` threads of which this is number `tid`
+    __device__ __forceinline__ void slice(const Slice& sl, int tid, int threads) const {
+        ends(sl, tid);
+        const uint4* zv = reinterpret_cast<const uint4*>(z + sl.body);
+        for (int i = sl.lo + tid; i < sl.hi; i += threads) vec(sl.body, i, u == 0.f ? make_uint4(0, 0, 0, 0) : zv[i]);
+    }
+    __device__ __forceinline__ void ends(const Slice& sl, int tid) const {
+        if (tid < sl.head) one(tid);
+        if (tid < sl.tail) one(sl.tail_at + tid);
+    }
+};
 
-        const float r = a.old_logp.p ? expf(logp - old) : (logp == logp ? 1.f : logp);   // NaN logits show in the loss
-        const bool clipped = (A > 0.f && r > 1.f + a.clip_high) || (A < 0.f && r < 1.f - a.clip_low);
-        const float gain = A == 0.f ? 0.f : (clipped ? (A > 0.f ? 1.f + a.clip_high : 1.f - a.clip_low) : r) * A;
-        float dl = clipped ? 0.f : -gain, k = 0.f;
-        if (a.ref_logp.p) {
-            const float x = ref - logp, e = expm1f(x);
-            k = e - x;
-            dl -= a.kl_coef * e;
-        }
-        const float u = float(double(w) * inv_d * double(dl) / double(a.temperature));
-        if (rank == 0 && tid == 0) {
-            a.logp[row] = logp;
-            saved_of(a)[row] = make_float4(u, R, s, far ? 1.f : 0.f);
-            loss += double(w) * (double(a.ref_logp.p ? a.kl_coef * k : 0.f) - double(gain));
-            kl += double(w) * double(k);
-            cut += clipped ? double(w) : 0.0;
-        }
-        if (GRAD) write_grad<T>(z, g, sl, V, token, u, R, s, c, far);
-    }
-    if (rank == 0 && tid == 0) {
-        double* p = partials_of(a) + 3 * (blockIdx.x / C);
-        p[0] = loss;
-        p[1] = kl;
-        p[2] = cut;
-    }
+// What a row needs besides its logits.
+struct RowIn {
+    int64_t row, at, grad_at, token;
+    float w, advantage, old, ref;
+};
+__device__ __forceinline__ RowIn row_in(const crx_policy_args& a, int64_t row) {
+    const int64_t b = row / a.steps, t = row - b * a.steps;
+    RowIn r;
+    r.row = row;
+    r.at = at(a.logits, b, t);
+    r.grad_at = at(a.grad, b, t);
+    r.token = a.tokens64 ? static_cast<const int64_t*>(a.tokens.p)[at(a.tokens, b, t)]
+                         : static_cast<const int32_t*>(a.tokens.p)[at(a.tokens, b, t)];
+    r.w = weight(a, b, t);
+    r.advantage = value(a.advantages, b, t);
+    r.old = a.old_logp.p ? value(a.old_logp, b, t) : 0.f;
+    r.ref = a.ref_logp.p ? value(a.ref_logp, b, t) : 0.f;
+    return r;
 }
 
 __device__ __forceinline__ double warp_sum(double v) {
@@ -363,29 +338,282 @@ __device__ __forceinline__ double warp_sum(double v) {
     return v;
 }
 
-__global__ void __launch_bounds__(1024) k_policy_denom(const __grid_constant__ crx_policy_args a) {
-    __shared__ double red[32];
-    double v = 0;
-    for (int64_t i = threadIdx.x; i < a.batch * a.steps; i += 1024) {
-        const int64_t b = i / a.steps;
-        v += double(weight(a, b, i - b * a.steps));
+__device__ __forceinline__ uint32_t smem_of(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
+
+// Whether the phase `parity` of the barrier completed; gives up after some seconds, which only a
+// copy that never ends could bring about.
+__device__ __forceinline__ bool wait_full(uint32_t bar, uint32_t parity) {
+    for (int i = 0; i < (1 << 20); ++i) {
+        uint32_t ok;
+        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
     }
-    v = warp_sum(v);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        v = warp_sum(red[threadIdx.x]);
-        if (threadIdx.x == 0) *inv_denom_of(a) = v == 0.0 ? 0.0 : 1.0 / v;
+    return false;
+}
+
+// A warp's stream: the chunks of its part of every row that counts, in the plan's order (a row that does not
+// fit the ring comes twice, for the gradient).  `issued` chunks are on their way or here, the first
+// `freed` of them are done with.
+template <class T, bool GRAD, bool WARP>
+struct Stream {
+    const crx_policy_args& a;
+    uint32_t ring, bars;       // shared addresses: kSlots chunks, kSlots barriers
+    int64_t i, step, n;        // place of the row being issued among those that count, the unit's stride, their number
+    const int32_t* order;
+    int rank, C;
+    const char* from;          // its first vector
+    int lo, hi, at_vec, again; // its vectors, the next one, times it is still to come after this one
+    uint32_t issued = 0, freed = 0;
+
+    static constexpr int kStride = WARP ? kChunk : kChunk * kRowWarps;
+
+    __device__ __forceinline__ Stream(const crx_policy_args& a, char* mem, uint64_t* bars_, int64_t i, int64_t step, int64_t n,
+                                      const int32_t* order, int rank, int C)
+        : a(a), i(i), step(step), n(n), order(order), rank(rank), C(C) {
+        const int warp = threadIdx.x >> 5;
+        ring = smem_of(mem) + uint32_t(warp) * (kSlots * kChunk * 16);
+        bars = smem_of(bars_ + warp * kSlots);
+        open();
+    }
+    // the warp's vectors of a slice, as its first one and its chunks
+    static __device__ __forceinline__ int first(const Slice& sl) { return sl.lo + (WARP ? 0 : int(threadIdx.x >> 5) * kChunk); }
+    static __device__ __forceinline__ int chunks(const Slice& sl) {
+        const int left = sl.hi - first(sl);
+        return left > 0 ? (left + kStride - 1) / kStride : 0;
+    }
+    // goes on to the next row that has a part for this warp
+    __device__ __forceinline__ void open() {
+        for (; i < n; i += step) {
+            const int64_t row = order ? order[i] : i, b = row / a.steps, t = row - b * a.steps;
+            const T* z = static_cast<const T*>(a.logits.p) + at(a.logits, b, t);
+            const Slice sl = slice_of<T>(z, a.vocab, rank, C);
+            const int k = chunks(sl);
+            if (!k) continue;
+            from = reinterpret_cast<const char*>(z + sl.body);
+            lo = at_vec = first(sl);
+            hi = sl.hi;
+            again = GRAD && k > kSlots;
+            return;
+        }
+    }
+    __device__ __forceinline__ void fill() {
+        while (issued - freed < kSlots && i < n) {
+            if ((threadIdx.x & 31) == 0) {
+                const uint32_t slot = issued % kSlots, bytes = uint32_t(tmin(kChunk, hi - at_vec)) * 16;
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bars + slot * 8), "r"(bytes) : "memory");
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                                 ring + slot * (kChunk * 16)),
+                             "l"(from + int64_t(at_vec) * 16), "r"(bytes), "r"(bars + slot * 8)
+                             : "memory");
+            }
+            ++issued;
+            at_vec += kStride;
+            if (at_vec >= hi) {
+                if (again) {
+                    again = 0;
+                    at_vec = lo;
+                } else {
+                    i += step;
+                    open();
+                }
+            }
+        }
+    }
+    // the lane's vectors of chunk number `k` of the stream
+    __device__ __forceinline__ void read(uint32_t k, uint4* q) const {
+        const uint32_t p = ring + (k % kSlots) * (kChunk * 16) + (threadIdx.x & 31) * 16;
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q[v].x), "=r"(q[v].y), "=r"(q[v].z), "=r"(q[v].w) : "r"(p + v * 512) : "memory");
+    }
+    __device__ __forceinline__ bool wait(uint32_t k) const { return wait_full(bars + (k % kSlots) * 8, (k / kSlots) & 1); }
+    __device__ __forceinline__ void release() {
+        __syncwarp();   // every lane has its values
+        ++freed;
+        fill();
+    }
+};
+
+template <class T, bool GRAD, bool WARP>
+__global__ void __launch_bounds__(kRowThreads, kRowCtas) k_policy_rows(const __grid_constant__ crx_policy_args a, double inv_denom, int planned, int C) {
+    extern __shared__ __align__(128) char ring[];
+    __shared__ uint64_t bars[kRowWarps * kSlots];
+    __shared__ Shared sh;
+    const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, lane = threadIdx.x & 31, threads = WARP ? 32 : kRowThreads;
+    const int rank = WARP ? 0 : int(blockIdx.x) % C;
+    const int64_t n = a.batch * a.steps, V = a.vocab;
+    const int64_t unit = WARP ? int64_t(blockIdx.x) * kRowWarps + (threadIdx.x >> 5) : blockIdx.x / C;
+    const int64_t units = WARP ? int64_t(gridDim.x) * kRowWarps : gridDim.x / C;
+    if (threadIdx.x < kRowWarps * kSlots)
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_of(&bars[threadIdx.x])) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;\nfence.proxy.async.shared::cta;" ::: "memory");
+    if (!WARP && C > 1) cg::this_cluster().sync();   // every CTA runs before another writes to its shared memory
+    else __syncthreads();
+    const float c = float(1.4426950408889634 / double(a.temperature));
+    const float inv_d = float(inv_denom < 0 ? plan_of(a)->inv_denom : inv_denom), inv_tau = 1.f / a.temperature;
+    const int32_t* order = planned ? order_of(a) : nullptr;
+    const int64_t counted = planned ? plan_of(a)->counted : n;
+    double loss = 0, kl = 0, cut = 0;
+    int parity = 0;
+    Stream<T, GRAD, WARP> in(a, ring, bars, unit, units, counted, order, rank, C);
+    in.fill();
+    RowIn next;
+    if (unit < n) next = row_in(a, order ? order[unit] : unit);
+    for (int64_t i = unit; i < n; i += units) {
+        const RowIn r = next;
+        const float w = r.w;
+        const int64_t row = r.row;
+        const T* z = static_cast<const T*>(a.logits.p) + r.at;
+        T* g = GRAD ? static_cast<T*>(const_cast<void*>(a.grad.p)) + r.grad_at : nullptr;
+        const Slice sl = slice_of<T>(z, V, rank, C);
+        const float za = i < counted && r.token >= 0 && r.token < V ? to_f(z[r.token]) : NAN;
+        if (i + units < n) next = row_in(a, order ? order[i + units] : i + units);   // (its latency passes under this row)
+        if (i >= counted) {
+            if (GRAD) GradOf<T>(z, g, sl, -1, 0.f, 0.f, 1.f, c, false).slice(sl, tid, threads);
+            if (rank == 0 && tid == 0) {
+                a.logp[row] = 0.f;
+                saved_of(a)[row] = make_float4(0.f, 0.f, 1.f, 0.f);
+            }
+            continue;
+        }
+
+        Running run;
+        const auto one = [&](int j) {
+            const float x = to_f(z[j]);
+            run.raise(x, c);
+            run.s += exp2_fast(fmaf(x, c, -run.r));
+        };
+        if (tid < sl.head) one(tid);
+        if (tid < sl.tail) one(sl.tail_at + tid);
+        const int first = in.first(sl), chunks = in.chunks(sl);
+        const bool fits = chunks <= kSlots;
+        const uint32_t base = in.freed;
+        bool came = true;
+        for (int k = 0; k < chunks; ++k) {
+            uint4 q[4];
+            came &= in.wait(base + k);
+            in.read(base + k, q);
+            const int v0 = first + k * in.kStride + lane;
+            if (v0 + 96 >= sl.hi) {   // the last chunk: what lies behind the slice adds nothing
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+                    if (v0 + 32 * v >= sl.hi) q[v] = Vec<T>::lowest();
+            }
+            add_vecs<T, 4>(q, run, c);
+            if (!GRAD || !fits) in.release();
+        }
+        if (!came) run.s = NAN;
+        run = row_total<WARP>(run, sh, parity, rank, C, c);
+        parity ^= 1;
+        const bool far = fabsf(run.m) <= 3.402823466e38f && !(fabsf(run.m * c) < kFar);
+        const float s = far ? far_sum<T, WARP>(z, V, run.m, c, sh) : run.s;
+        const float R = far ? run.m : run.r;
+        const float logp = ((far ? (za - R) * c : fmaf(za, c, -R)) - log2f(s)) * 0.6931471805599453f;
+
+        const float A = r.advantage;
+        const float ratio = a.old_logp.p ? expf(logp - r.old) : (logp == logp ? 1.f : logp);   // NaN logits show in the loss
+        const bool clipped = (A > 0.f && ratio > 1.f + a.clip_high) || (A < 0.f && ratio < 1.f - a.clip_low);
+        const float gain = A == 0.f ? 0.f : (clipped ? (A > 0.f ? 1.f + a.clip_high : 1.f - a.clip_low) : ratio) * A;
+        float dl = clipped ? 0.f : -gain, k = 0.f;
+        if (a.ref_logp.p) {
+            const float x = r.ref - logp, e = expm1f(x);
+            k = e - x;
+            dl -= a.kl_coef * e;
+        }
+        const float u = w * inv_d * dl * inv_tau;
+        if (rank == 0 && tid == 0) {
+            a.logp[row] = logp;
+            saved_of(a)[row] = make_float4(u, R, s, far ? 1.f : 0.f);
+            loss += double(w * (a.kl_coef * k - gain));
+            kl += double(w * k);
+            cut += double(clipped ? w : 0.f);
+        }
+        if (GRAD) {
+            const GradOf<T> grad(z, g, sl, r.token, u, R, s, c, far);
+            grad.ends(sl, tid);
+            const uint32_t from = in.freed;
+            for (int k = 0; k < chunks; ++k) {
+                uint4 q[4];
+                if (!fits) in.wait(from + k);
+                in.read(from + k, q);
+                const int v0 = first + k * in.kStride + lane;
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+                    if (v0 + 32 * v < sl.hi) grad.vec(sl.body, v0 + 32 * v, q[v]);
+                in.release();
+            }
+        }
+    }
+    if (rank == 0 && tid == 0) {
+        double* p = partials_of(a) + 3 * unit;
+        p[0] = loss;
+        p[1] = kl;
+        p[2] = cut;
     }
 }
 
-// Warp i sums term i.
-__global__ void __launch_bounds__(96) k_policy_sums(const __grid_constant__ crx_policy_args a, double inv_denom, int clusters) {
-    const int i = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// Every thread takes a run of rows; the counts before it give it its places among the rows that
+// count and among those that do not.
+__global__ void __launch_bounds__(1024) k_policy_plan(const __grid_constant__ crx_policy_args a) {
+    __shared__ double red[32];
+    __shared__ int before[32];
+    const int n = int(a.batch * a.steps), steps = int(a.steps), tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+    const int per = (n + 1023) / 1024;
+    const int lo = int(tmin<int64_t>(n, int64_t(tid) * per)), hi = int(tmin<int64_t>(n, int64_t(lo) + per));
     double v = 0;
-    for (int k = lane; k < clusters; k += 32) v += partials_of(a)[3 * k + i];
-    v = warp_sum(v) * (inv_denom < 0 ? *inv_denom_of(a) : inv_denom);
-    if (lane == 0) *(i ? a.stats + i - 1 : a.loss) = float(v);
+    int c = 0;
+    for (int i = lo; i < hi; ++i) {
+        const float x = weight(a, i / steps, i % steps);
+        v += double(x);
+        c += x != 0.f;
+    }
+    v = warp_sum(v);
+    int incl = c;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+    }
+    if (lane == 31) before[w] = incl;
+    if (lane == 0) red[w] = v;
+    __syncthreads();
+    const int mine = before[lane];
+    int total = mine, scan = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, scan, o);
+        if (lane >= o) scan += y;
+    }
+    total = __shfl_sync(0xffffffffu, scan, 31);
+    int in = __shfl_sync(0xffffffffu, scan - mine, w) + incl - c;   // rows that count before this thread's
+    int out = total + lo - in;
+    int32_t* order = order_of(a);
+    for (int i = lo; i < hi; ++i) {
+        if (weight(a, i / steps, i % steps) != 0.f) order[in++] = i;
+        else order[out++] = i;
+    }
+    if (w == 0) {
+        v = warp_sum(red[lane]);
+        if (lane == 0) {
+            plan_of(a)->inv_denom = v == 0.0 ? 0.0 : 1.0 / v;
+            plan_of(a)->counted = total;
+        }
+    }
+}
+
+__global__ void __launch_bounds__(768) k_policy_sums(const __grid_constant__ crx_policy_args a, double inv_denom, int units) {
+    __shared__ double red[24];
+    const int w = threadIdx.x >> 5, i = w >> 3, lane = threadIdx.x & 31;   // eight warps per term
+    double v = 0;
+    for (int k = threadIdx.x & 255; k < units; k += 256) v += partials_of(a)[3 * k + i];
+    v = warp_sum(v);
+    if (lane == 0) red[w] = v;
+    __syncthreads();
+    if (threadIdx.x < 3) {
+        v = 0;
+        for (int k = 0; k < 8; ++k) v += red[8 * threadIdx.x + k];
+        v *= inv_denom < 0 ? plan_of(a)->inv_denom : inv_denom;
+        *(threadIdx.x ? a.stats + threadIdx.x - 1 : a.loss) = float(v);
+    }
 }
 
 // The gradient again for a scale other than the one it was written with.  CTAs take (row, slice)
@@ -405,7 +633,8 @@ __global__ void __launch_bounds__(kRowThreads) k_policy_again(const __grid_const
         const int64_t token = a.tokens64 ? static_cast<const int64_t*>(a.tokens.p)[at(a.tokens, b, t)]
                                          : static_cast<const int32_t*>(a.tokens.p)[at(a.tokens, b, t)];
         const float u = saved.x == 0.f ? 0.f : saved.x * f;   // a row that does not count stays 0 whatever the scale
-        write_grad<T>(z, g, slice_of<T>(z, a.vocab, int(item - row * C), C), a.vocab, token, u, saved.y, saved.z, c, saved.w != 0.f);
+        const Slice sl = slice_of<T>(z, a.vocab, int(item - row * C), C);
+        GradOf<T>(z, g, sl, token, u, saved.y, saved.z, c, saved.w != 0.f).slice(sl, threadIdx.x, kRowThreads);
     }
 }
 
@@ -416,38 +645,65 @@ int fail(char* err, size_t errlen, int status, const std::string& msg) {
     return status;
 }
 
-constexpr int kRowGrid = 148 * 2;   // CTAs of the persistent grid
-constexpr int kMaxClusters = kRowGrid;
+// A row by one warp, where its ring holds one: no warp waits for another.
+bool warp_rows(int64_t n, int64_t V, int vec) { return V <= int64_t(kSlots) * kChunk * vec && n >= kRowGrid; }
 
-// CTAs per row: as many as the rows leave room for, while a slice keeps 2048 elements.
-int cluster_for(int64_t n, int64_t V) {
+// CTAs per row: enough for the rings to hold one (with a gradient: its logits are then read once), and
+// as many as the rows leave room for while a slice keeps two chunks.
+int cluster_for(int64_t n, int64_t V, int vec, bool grad) {
     int C = 1;
-    while (C < kMaxCluster && n * C * 2 <= kRowGrid && V >= 2048 * 2 * C) C *= 2;
+    while (C < kMaxCluster && ((grad && V > int64_t(kRowWarps) * kSlots * kChunk * vec * C) || (n * C * 2 <= kRowGrid && V >= int64_t(kChunk) * vec * 4 * C)))
+        C *= 2;
     return C;
 }
 
-template <class T, bool GRAD>
-cudaError_t launch_rows(const crx_policy_args& a, double inv_denom, int* clusters, cudaStream_t st) {
-    const int64_t n = a.batch * a.steps;
-    const int C = cluster_for(n, a.vocab);
-    *clusters = int(std::min<int64_t>(n, kRowGrid / C));
+template <class T, bool GRAD, bool WARP>
+cudaError_t launch_as(const crx_policy_args& a, double inv_denom, int C, int64_t most, int* units, cudaStream_t st) {
+    const auto kernel = k_policy_rows<T, GRAD, WARP>;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(*clusters * C));
     cfg.blockDim = dim3(kRowThreads);
+    cfg.gridDim = dim3(kRowGrid / C * C);
+    cfg.dynamicSmemBytes = kRingBytes;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = unsigned(C);
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = C > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, k_policy_rows<T, GRAD>, a, inv_denom, C);
+    cfg.numAttrs = 1;
+    // clusters that run at once: those of four and eight do not fill every GPC, and rows dealt to more
+    // would wait for a second round
+    static std::atomic<int> fit[kMaxDevices][4];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= kMaxDevices) return cudaErrorInvalidDevice;
+    std::atomic<int>& known = fit[dev][C == 1 ? 0 : C == 2 ? 1 : C == 4 ? 2 : 3];
+    int clusters = known.load(std::memory_order_relaxed);
+    if (!clusters) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kRingBytes));
+        if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg);
+        if (e != cudaSuccess) return e;
+        clusters = std::max(1, std::min(clusters, kRowGrid / C));
+        known.store(clusters, std::memory_order_relaxed);
+    }
+    const int grid = int(std::min<int64_t>(most, clusters));
+    *units = WARP ? grid * kRowWarps : grid;
+    cfg.gridDim = dim3(unsigned(grid * C));
+    return cudaLaunchKernelEx(&cfg, kernel, a, inv_denom, int(a.mask.p != nullptr), C);
+}
+
+template <class T, bool GRAD>
+cudaError_t launch_rows(const crx_policy_args& a, double inv_denom, int* units, cudaStream_t st) {
+    const int64_t n = a.batch * a.steps;
+    if (warp_rows(n, a.vocab, Vec<T>::N)) return launch_as<T, GRAD, true>(a, inv_denom, 1, (n + kRowWarps - 1) / kRowWarps, units, st);
+    return launch_as<T, GRAD, false>(a, inv_denom, cluster_for(n, a.vocab, Vec<T>::N, GRAD), n, units, st);
 }
 
 template <class T>
 cudaError_t launch_again(const crx_policy_args& a, const float* scale, int unless_one, cudaStream_t st) {
     const int64_t n = a.batch * a.steps;
-    const int C = cluster_for(n, a.vocab);
+    const int C = cluster_for(n, a.vocab, Vec<T>::N, true);
     k_policy_again<T><<<unsigned(std::min<int64_t>(n * C, kRowGrid * 2)), kRowThreads, 0, st>>>(a, scale, unless_one, C);
     return cudaGetLastError();
 }
@@ -456,7 +712,7 @@ int check(const char* who, const crx_policy_args* a, char* err, size_t errlen) {
     const auto bad = [&](const char* what) { return fail(err, errlen, CRX_BAD_ARGUMENT, std::string(who) + ": " + what); };
     if (!a) return bad("null arguments");
     if (a->batch < 0 || a->steps < 0 || a->vocab < 1 || a->vocab > (int64_t(1) << 31) || a->batch > (int64_t(1) << 31) || a->steps > (int64_t(1) << 31) ||
-        (a->batch && a->steps > (int64_t(1) << 40) / a->batch))
+        (a->batch && a->steps >= (int64_t(1) << 31) / a->batch))
         return bad("size out of range");
     if (a->dtype != CRX_BF16 && a->dtype != CRX_FP16 && a->dtype != CRX_FP32) return bad("unknown type");
     const uintptr_t es = a->dtype == CRX_FP32 ? 4 : 2;
@@ -479,7 +735,7 @@ extern "C" {
 
 int64_t crx_policy_workspace(int64_t batch, int64_t steps) {
     if (batch < 0 || steps < 0) return 0;
-    return 16 + 16 * batch * steps + int64_t(sizeof(double)) * 3 * kMaxClusters;
+    return 16 + 20 * batch * steps + int64_t(sizeof(double)) * 3 * kMaxUnits;
 }
 
 int crx_policy_loss(const crx_policy_args* args, void* stream, char* err, size_t errlen) {
@@ -494,21 +750,21 @@ int crx_policy_loss(const crx_policy_args* args, void* stream, char* err, size_t
             if (e == cudaSuccess) e = cudaMemsetAsync(a.stats, 0, 2 * sizeof(float), st);
             return e == cudaSuccess ? CRX_OK : fail(err, errlen, CRX_CUDA_ERROR, std::string("crx_policy_loss: ") + cudaGetErrorString(e));
         }
-        // a negative 1 / denominator: the kernels take the one that k_policy_denom wrote
+        // a negative 1 / denominator: the kernels take the plan's
         const double inv_denom = a.denom > 0 ? 1.0 / a.denom : a.mask.p ? -1.0 : 1.0 / double(n);
-        if (inv_denom < 0) {
-            k_policy_denom<<<1, 1024, 0, st>>>(a);
+        if (a.mask.p) {
+            k_policy_plan<<<1, 1024, 0, st>>>(a);
             e = cudaGetLastError();
         }
-        int clusters = 0;
+        int units = 0;
         const bool grad = a.grad.p != nullptr;
         if (e == cudaSuccess) {
-            if (a.dtype == CRX_BF16) e = grad ? launch_rows<__nv_bfloat16, true>(a, inv_denom, &clusters, st) : launch_rows<__nv_bfloat16, false>(a, inv_denom, &clusters, st);
-            else if (a.dtype == CRX_FP16) e = grad ? launch_rows<__half, true>(a, inv_denom, &clusters, st) : launch_rows<__half, false>(a, inv_denom, &clusters, st);
-            else e = grad ? launch_rows<float, true>(a, inv_denom, &clusters, st) : launch_rows<float, false>(a, inv_denom, &clusters, st);
+            if (a.dtype == CRX_BF16) e = grad ? launch_rows<__nv_bfloat16, true>(a, inv_denom, &units, st) : launch_rows<__nv_bfloat16, false>(a, inv_denom, &units, st);
+            else if (a.dtype == CRX_FP16) e = grad ? launch_rows<__half, true>(a, inv_denom, &units, st) : launch_rows<__half, false>(a, inv_denom, &units, st);
+            else e = grad ? launch_rows<float, true>(a, inv_denom, &units, st) : launch_rows<float, false>(a, inv_denom, &units, st);
         }
         if (e == cudaSuccess) {
-            k_policy_sums<<<1, 96, 0, st>>>(a, inv_denom, clusters);
+            k_policy_sums<<<1, 768, 0, st>>>(a, inv_denom, units);
             e = cudaGetLastError();
         }
         return e == cudaSuccess ? CRX_OK : fail(err, errlen, CRX_CUDA_ERROR, std::string("crx_policy_loss: ") + cudaGetErrorString(e));
