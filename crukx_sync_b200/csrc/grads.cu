@@ -20,11 +20,14 @@
 #include <cstring>
 #include <exception>
 #include <string>
+#include <type_traits>
+#include <utility>
 #include <vector>
 
 #include "../../include/crukx_b200.h"
 #include "common.cuh"
 #include "elements.cuh"
+#include "launch.cuh"
 
 namespace crx {
 namespace {
@@ -169,6 +172,7 @@ __global__ void __launch_bounds__(kThreads) k_grad_sumsq(const __grid_constant__
         else if (t.e[i].dtype == CRX_BF16) tile_sumsq(static_cast<const __nv_bfloat16*>(t.e[i].g), t.e[i].numel, k, acc);
         else tile_sumsq(static_cast<const __half*>(t.e[i].g), t.e[i].numel, k, acc);
     }
+    let_next_start();
     acc = block_sum(acc, red);
     if (threadIdx.x == 0) partials[blockIdx.x] = acc;
 }
@@ -181,6 +185,8 @@ __device__ __forceinline__ double sum_partials(const double* __restrict__ partia
 
 __global__ void __launch_bounds__(kThreads) k_grad_norm(const double* __restrict__ partials, int n, float* __restrict__ norm) {
     __shared__ double red[kThreads / 32];
+    after_previous();
+    let_next_start();
     const double s = sum_partials(partials, n, red);
     if (threadIdx.x == 0) *norm = float(sqrt(s));
 }
@@ -234,6 +240,7 @@ __global__ void __launch_bounds__(kThreads) k_grad_clip(const __grid_constant__ 
                                                         int n_partials, const float* __restrict__ norm_in, float max_norm,
                                                         float* __restrict__ norm_out) {
     __shared__ double red[kThreads / 32];
+    after_previous();
     const float norm = n_partials ? float(sqrt(sum_partials(partials, n_partials, red))) : *norm_in;
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
     const float c = clip_coef(norm, max_norm);
@@ -501,8 +508,8 @@ int crx_grad_norm(int32_t n, const void* const* grads, const int32_t* dtypes, co
         int count = 0;
         cudaError_t e = launch_sumsq(n, grads, dtypes, numel, partials, &count, st);
         if (e == cudaSuccess) {
-            k_grad_norm<<<1, kThreads, 0, st>>>(partials, count, norm);
-            e = cudaGetLastError();
+            e = count ? launch_behind(k_grad_norm, 1, kThreads, st, static_cast<const double*>(partials), count, norm)
+                      : cudaMemsetAsync(norm, 0, sizeof(float), st);
         }
         return e == cudaSuccess ? CRX_OK : cuda_fail(err, errlen, "crx_grad_norm", e);
     } catch (const std::exception& ex) {
@@ -538,9 +545,9 @@ int crx_clip_grads(int32_t n, const void* const* grads, void* const* out, const 
         int count = 0;
         cudaError_t e = norm_in ? cudaSuccess : launch_sumsq(n, grads, dtypes, numel, partials, &count, st);
         float* write_norm = norm_out;   // by the first launch that knows it
+        bool behind = norm_in == nullptr;
         if (e == cudaSuccess && count > kClipPartials) {
-            k_grad_norm<<<1, kThreads, 0, st>>>(partials, count, norm_out);
-            e = cudaGetLastError();
+            e = launch_behind(k_grad_norm, 1, kThreads, st, static_cast<const double*>(partials), count, norm_out);
             norm_in = norm_out;
             write_norm = nullptr;
             count = 0;
@@ -556,8 +563,12 @@ int crx_clip_grads(int32_t n, const void* const* grads, void* const* out, const 
                     return grad_tiles(grads[i], numel[i], dtypes[i]);
                 },
                 [&](const auto& t) {
-                    k_grad_clip<<<t.tiles, kThreads, 0, st>>>(t, partials, count, norm_in, max_norm, write_norm);
+                    using Tab = std::decay_t<decltype(t)>;
+                    float* const w = write_norm;
                     write_norm = nullptr;
+                    if (std::exchange(behind, false))
+                        return launch_behind(k_grad_clip<Tab>, t.tiles, kThreads, st, t, static_cast<const double*>(partials), count, norm_in, max_norm, w);
+                    k_grad_clip<<<t.tiles, kThreads, 0, st>>>(t, partials, count, norm_in, max_norm, w);
                     return cudaGetLastError();
                 });
         if (e == cudaSuccess && write_norm) {   // no elements at all

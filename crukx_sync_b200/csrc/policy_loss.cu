@@ -29,16 +29,17 @@
 #include "../../include/crukx_b200.h"
 #include "common.cuh"
 #include "elements.cuh"
+#include "launch.cuh"
 
 namespace crx {
 namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kRowThreads = 256;
+constexpr int kRowThreads = 128;
 constexpr int kRowWarps = kRowThreads / 32;
 constexpr int kMaxCluster = 8;
-constexpr int kRowCtas = 2;            // per SM
+constexpr int kRowCtas = 4;            // per SM
 constexpr int kSlots = 6;              // of a warp's ring
 constexpr int kChunk = 128;            // 16-byte vectors of a slot: four per lane
 constexpr int kRowGrid = 148 * kRowCtas;       // CTAs of the persistent grid
@@ -131,20 +132,27 @@ struct Running {
     }
 };
 
+// 2^(x c + d) of both values.
+__device__ __forceinline__ f32x2 exp2_pair(f32x2 x, f32x2 c, f32x2 d) {
+    float a, b;
+    unpack2(fma2(x, c, d), a, b);
+    return pack2(exp2_fast(a), exp2_fast(b));
+}
+
 template <class T, int U>
 __device__ __forceinline__ void add_vecs(const uint4* q, Running& run, float c) {
     run.raise(vec_max<T>(q, U), c);
-    float a = 0.f, b = 0.f;
+    const f32x2 cc = pack2(c, c), d = pack2(-run.r, -run.r);
+    f32x2 sum[2] = {0, 0};
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         float x[Vec<T>::N];
         Vec<T>::get(q[u], x);
 #pragma unroll
-        for (int i = 0; i < Vec<T>::N; i += 2) {
-            a += exp2_fast(fmaf(x[i], c, -run.r));
-            b += exp2_fast(fmaf(x[i + 1], c, -run.r));
-        }
+        for (int i = 0; i < Vec<T>::N; i += 2) sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], exp2_pair(pack2(x[i], x[i + 1]), cc, d));
     }
+    float a, b;
+    unpack2(add2(sum[0], sum[1]), a, b);
     run.s += a + b;
 }
 
@@ -171,9 +179,24 @@ __device__ __forceinline__ Slice slice_of(const T* z, int64_t V, int rank, int C
 }
 
 struct Shared {
-    float2 warp[kRowWarps];
-    float2 part[2][kMaxCluster];   // (M, s) of every CTA of the cluster, double-buffered over rows
+    float2 warp[2][kRowWarps];     // (M, s) of every warp, double-buffered over rows
+    float2 part[2][kMaxCluster];   // and of every CTA of the cluster
+    uint64_t came[2];              // barriers: the cluster's parts are here
 };
+
+__device__ __forceinline__ uint32_t smem_of(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
+
+// Whether the phase `parity` of the barrier completed; gives up after some seconds, which only a
+// copy that never ends could bring about.
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity) {
+    for (int i = 0; i < (1 << 20); ++i) {
+        uint32_t ok;
+        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
 
 // The largest of a warp's values: as integers of the same order, one instruction for the warp.
 __device__ __forceinline__ float warp_max(float x) {
@@ -204,26 +227,35 @@ __device__ __forceinline__ Running lane_entry(const float2* e, int n) {
     return r;
 }
 
-// (M, s) of the whole row from every thread's; the same bits in every thread of the cluster.
+// (M, s) of the whole row number `i` of the unit from every thread's; the same bits in every thread.
+// The CTAs of a cluster send their parts into each other's shared memory, counted in by a barrier
+// there: a cluster barrier would also wait for the stores of the row before.  A CTA cannot be two
+// rows ahead of another, whose part of the row between it needs, so two buffers are enough.
 template <bool WARP>
-__device__ __forceinline__ Running row_total(Running run, Shared& sh, int parity, int rank, int C, float c) {
+__device__ __forceinline__ Running row_total(Running run, Shared& sh, uint32_t i, int rank, int C, float c) {
     run = warp_total(run, c);
     if (WARP) return run;
-    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (lane == 0) sh.warp[w] = make_float2(run.m, run.s);
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, half = i & 1;
+    if (lane == 0) sh.warp[half][w] = make_float2(run.m, run.s);
     __syncthreads();
-    if (C == 1) {
-        run = warp_total(lane_entry(sh.warp, kRowWarps), c);
-        __syncthreads();   // sh.warp is written again by the next row
-        return run;
-    }
-    cg::cluster_group cl = cg::this_cluster();
+    if (C == 1) return warp_total(lane_entry(sh.warp[half], kRowWarps), c);
+    const uint32_t came = smem_of(&sh.came[half]);
     if (w == 0) {
-        run = warp_total(lane_entry(sh.warp, kRowWarps), c);
-        if (lane < C) *cl.map_shared_rank(&sh.part[parity][rank], lane) = make_float2(run.m, run.s);
+        run = warp_total(lane_entry(sh.warp[half], kRowWarps), c);
+        if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(came), "r"(C * 8) : "memory");
+        if (lane < C) {
+            uint32_t to, bar;
+            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_of(&sh.part[half][rank])), "r"(lane));
+            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(came), "r"(lane));
+            asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(to), "f"(run.m), "f"(run.s),
+                         "r"(bar)
+                         : "memory");
+        }
     }
-    cl.sync();
-    return warp_total(lane_entry(sh.part[parity], C), c);
+    const bool here = wait_phase(came, (i >> 1) & 1);
+    run = warp_total(lane_entry(sh.part[half], C), c);
+    if (!here) run.s = NAN;
+    return run;
 }
 
 template <bool WARP>
@@ -231,10 +263,10 @@ __device__ __forceinline__ float unit_total(float v, Shared& sh) {
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (WARP) return v;
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5].y = v;
+    if ((threadIdx.x & 31) == 0) sh.warp[0][threadIdx.x >> 5].y = v;
     __syncthreads();
     v = 0.f;
-    for (int k = 0; k < kRowWarps; ++k) v += sh.warp[k].y;
+    for (int k = 0; k < kRowWarps; ++k) v += sh.warp[0][k].y;
     __syncthreads();
     return v;
 }
@@ -261,8 +293,8 @@ struct GradOf {
     bool far, wide;   // wide: gradient rows start at the same place between 16-byte boundaries as the logits'
     int token_vec;
 
-    __device__ __forceinline__ GradOf(const T* z, T* g, const Slice& sl, int64_t token, float u, float R, float s, float c, bool far)
-        : z(z), g(g), token(token), u(u), k(u == 0.f ? 0.f : u / s), R(R), c(c), far(far) {
+    __device__ __forceinline__ GradOf(const T* z, T* g, const Slice& sl, int64_t V, int64_t token_, float u, float R, float s, float c, bool far)
+        : z(z), g(g), token(token_ >= 0 && token_ < V ? token_ : -1), u(u), k(u == 0.f ? 0.f : u / s), R(R), c(c), far(far) {
         wide = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
         token_vec = token >= sl.body ? int((token - sl.body) / N) : -1;
     }
@@ -301,6 +333,16 @@ struct GradOf {
         else
             for (int e = 0; e < N; ++e) o[e] = from_f<T>(x[e]);
     }
+    __device__ __forceinline__ bool plain() const { return wide && !far && u != 0.f; }
+    // the same where plain(), without the token: its lane puts that right afterwards
+    __device__ __forceinline__ void vec_plain(uint4* o, const uint4& q) const {
+        const f32x2 cc = pack2(c, c), d = pack2(-R, -R), kk = pack2(-k, -k);
+        float x[N];
+        Vec<T>::get(q, x);
+#pragma unroll
+        for (int e = 0; e < N; e += 2) unpack2(mul2(exp2_pair(pack2(x[e], x[e + 1]), cc, d), kk), x[e], x[e + 1]);
+        *o = Vec<T>::put(x);
+    }
     // a slice from global memory, by `threads` threads of which this is number `tid`
     __device__ __forceinline__ void slice(const Slice& sl, int tid, int threads) const {
         ends(sl, tid);
@@ -338,23 +380,19 @@ __device__ __forceinline__ double warp_sum(double v) {
     return v;
 }
 
-__device__ __forceinline__ uint32_t smem_of(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
-
-// Whether the phase `parity` of the barrier completed; gives up after some seconds, which only a
-// copy that never ends could bring about.
-__device__ __forceinline__ bool wait_full(uint32_t bar, uint32_t parity) {
-    for (int i = 0; i < (1 << 20); ++i) {
-        uint32_t ok;
-        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
-                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-        if (ok) return true;
+// A place in a warp's ring, and the phase of its barrier that says that the chunk is here.
+struct Place {
+    uint32_t slot = 0, phase = 0;
+    __device__ __forceinline__ void next() {
+        if (++slot == kSlots) {
+            slot = 0;
+            phase ^= 1;
+        }
     }
-    return false;
-}
+};
 
-// A warp's stream: the chunks of its part of every row that counts, in the plan's order (a row that does not
-// fit the ring comes twice, for the gradient).  `issued` chunks are on their way or here, the first
-// `freed` of them are done with.
+// A warp's stream: the chunks of its part of every row that counts, in the plan's order (a row that
+// does not fit the ring comes twice, for the gradient).
 template <class T, bool GRAD, bool WARP>
 struct Stream {
     const crx_policy_args& a;
@@ -362,9 +400,10 @@ struct Stream {
     int64_t i, step, n;        // place of the row being issued among those that count, the unit's stride, their number
     const int32_t* order;
     int rank, C;
-    const char* from;          // its first vector
-    int lo, hi, at_vec, again; // its vectors, the next one, times it is still to come after this one
-    uint32_t issued = 0, freed = 0;
+    const char* from;          // its next vector
+    int left, span, again;     // vectors still to come, of how many, and whether all of them once more
+    uint32_t to = 0;           // the slot that is filled next
+    Place at_;                 // the first chunk that is not done with
 
     static constexpr int kStride = WARP ? kChunk : kChunk * kRowWarps;
 
@@ -375,6 +414,7 @@ struct Stream {
         ring = smem_of(mem) + uint32_t(warp) * (kSlots * kChunk * 16);
         bars = smem_of(bars_ + warp * kSlots);
         open();
+        for (int k = 0; k < kSlots; ++k) issue();
     }
     // the warp's vectors of a slice, as its first one and its chunks
     static __device__ __forceinline__ int first(const Slice& sl) { return sl.lo + (WARP ? 0 : int(threadIdx.x >> 5) * kChunk); }
@@ -388,50 +428,49 @@ struct Stream {
             const int64_t row = order ? order[i] : i, b = row / a.steps, t = row - b * a.steps;
             const T* z = static_cast<const T*>(a.logits.p) + at(a.logits, b, t);
             const Slice sl = slice_of<T>(z, a.vocab, rank, C);
-            const int k = chunks(sl);
-            if (!k) continue;
-            from = reinterpret_cast<const char*>(z + sl.body);
-            lo = at_vec = first(sl);
-            hi = sl.hi;
-            again = GRAD && k > kSlots;
+            span = left = sl.hi - first(sl);
+            if (left <= 0) continue;
+            from = reinterpret_cast<const char*>(z + sl.body) + int64_t(first(sl)) * 16;
+            again = GRAD && left > kSlots * kStride;
             return;
         }
     }
-    __device__ __forceinline__ void fill() {
-        while (issued - freed < kSlots && i < n) {
-            if ((threadIdx.x & 31) == 0) {
-                const uint32_t slot = issued % kSlots, bytes = uint32_t(tmin(kChunk, hi - at_vec)) * 16;
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bars + slot * 8), "r"(bytes) : "memory");
-                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                                 ring + slot * (kChunk * 16)),
-                             "l"(from + int64_t(at_vec) * 16), "r"(bytes), "r"(bars + slot * 8)
-                             : "memory");
-            }
-            ++issued;
-            at_vec += kStride;
-            if (at_vec >= hi) {
-                if (again) {
-                    again = 0;
-                    at_vec = lo;
-                } else {
-                    i += step;
-                    open();
-                }
-            }
+    // the next chunk into the slot that has come free
+    __device__ __forceinline__ void issue() {
+        if (i >= n) return;
+        if ((threadIdx.x & 31) == 0) {
+            const uint32_t bytes = uint32_t(tmin(kChunk, left)) * 16, bar = bars + to * 8;
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                             ring + to * (kChunk * 16)),
+                         "l"(from), "r"(bytes), "r"(bar)
+                         : "memory");
+        }
+        to = to + 1 == kSlots ? 0 : to + 1;
+        left -= kStride;
+        from += kStride * 16;
+        if (left > 0) return;
+        if (again) {
+            again = 0;
+            from -= int64_t(span - left) * 16;
+            left = span;
+        } else {
+            i += step;
+            open();
         }
     }
-    // the lane's vectors of chunk number `k` of the stream
-    __device__ __forceinline__ void read(uint32_t k, uint4* q) const {
-        const uint32_t p = ring + (k % kSlots) * (kChunk * 16) + (threadIdx.x & 31) * 16;
+    // the lane's vectors of a chunk
+    __device__ __forceinline__ void read(const Place& p, uint4* q) const {
+        const uint32_t s = ring + p.slot * (kChunk * 16) + (threadIdx.x & 31) * 16;
 #pragma unroll
         for (int v = 0; v < 4; ++v)
-            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q[v].x), "=r"(q[v].y), "=r"(q[v].z), "=r"(q[v].w) : "r"(p + v * 512) : "memory");
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q[v].x), "=r"(q[v].y), "=r"(q[v].z), "=r"(q[v].w) : "r"(s + v * 512) : "memory");
     }
-    __device__ __forceinline__ bool wait(uint32_t k) const { return wait_full(bars + (k % kSlots) * 8, (k / kSlots) & 1); }
+    __device__ __forceinline__ bool wait(const Place& p) const { return wait_phase(bars + p.slot * 8, p.phase); }
     __device__ __forceinline__ void release() {
         __syncwarp();   // every lane has its values
-        ++freed;
-        fill();
+        at_.next();
+        issue();
     }
 };
 
@@ -445,19 +484,20 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) k_policy_rows(const __g
     const int64_t n = a.batch * a.steps, V = a.vocab;
     const int64_t unit = WARP ? int64_t(blockIdx.x) * kRowWarps + (threadIdx.x >> 5) : blockIdx.x / C;
     const int64_t units = WARP ? int64_t(gridDim.x) * kRowWarps : gridDim.x / C;
-    if (threadIdx.x < kRowWarps * kSlots)
-        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_of(&bars[threadIdx.x])) : "memory");
+    if (threadIdx.x < kRowWarps * kSlots + 2)
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_of(threadIdx.x < kRowWarps * kSlots ? &bars[threadIdx.x] : &sh.came[threadIdx.x - kRowWarps * kSlots]))
+                     : "memory");
     asm volatile("fence.mbarrier_init.release.cluster;\nfence.proxy.async.shared::cta;" ::: "memory");
     if (!WARP && C > 1) cg::this_cluster().sync();   // every CTA runs before another writes to its shared memory
     else __syncthreads();
+    after_previous();
     const float c = float(1.4426950408889634 / double(a.temperature));
     const float inv_d = float(inv_denom < 0 ? plan_of(a)->inv_denom : inv_denom), inv_tau = 1.f / a.temperature;
     const int32_t* order = planned ? order_of(a) : nullptr;
     const int64_t counted = planned ? plan_of(a)->counted : n;
     double loss = 0, kl = 0, cut = 0;
-    int parity = 0;
+    uint32_t nth = 0;   // of the unit's rows that count
     Stream<T, GRAD, WARP> in(a, ring, bars, unit, units, counted, order, rank, C);
-    in.fill();
     RowIn next;
     if (unit < n) next = row_in(a, order ? order[unit] : unit);
     for (int64_t i = unit; i < n; i += units) {
@@ -470,7 +510,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) k_policy_rows(const __g
         const float za = i < counted && r.token >= 0 && r.token < V ? to_f(z[r.token]) : NAN;
         if (i + units < n) next = row_in(a, order ? order[i + units] : i + units);   // (its latency passes under this row)
         if (i >= counted) {
-            if (GRAD) GradOf<T>(z, g, sl, -1, 0.f, 0.f, 1.f, c, false).slice(sl, tid, threads);
+            if (GRAD) GradOf<T>(z, g, sl, V, -1, 0.f, 0.f, 1.f, c, false).slice(sl, tid, threads);
             if (rank == 0 && tid == 0) {
                 a.logp[row] = 0.f;
                 saved_of(a)[row] = make_float4(0.f, 0.f, 1.f, 0.f);
@@ -488,24 +528,23 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) k_policy_rows(const __g
         if (tid < sl.tail) one(sl.tail_at + tid);
         const int first = in.first(sl), chunks = in.chunks(sl);
         const bool fits = chunks <= kSlots;
-        const uint32_t base = in.freed;
         bool came = true;
-        for (int k = 0; k < chunks; ++k) {
+        Place p = in.at_;
+        for (int k = 0, left = sl.hi - first; k < chunks; ++k, left -= in.kStride) {
             uint4 q[4];
-            came &= in.wait(base + k);
-            in.read(base + k, q);
-            const int v0 = first + k * in.kStride + lane;
-            if (v0 + 96 >= sl.hi) {   // the last chunk: what lies behind the slice adds nothing
+            came &= in.wait(p);
+            in.read(p, q);
+            p.next();
+            if (left < kChunk) {   // what lies behind the slice adds nothing
 #pragma unroll
                 for (int v = 0; v < 4; ++v)
-                    if (v0 + 32 * v >= sl.hi) q[v] = Vec<T>::lowest();
+                    if (lane + 32 * v >= left) q[v] = Vec<T>::lowest();
             }
             add_vecs<T, 4>(q, run, c);
             if (!GRAD || !fits) in.release();
         }
         if (!came) run.s = NAN;
-        run = row_total<WARP>(run, sh, parity, rank, C, c);
-        parity ^= 1;
+        run = row_total<WARP>(run, sh, nth++, rank, C, c);
         const bool far = fabsf(run.m) <= 3.402823466e38f && !(fabsf(run.m * c) < kFar);
         const float s = far ? far_sum<T, WARP>(z, V, run.m, c, sh) : run.s;
         const float R = far ? run.m : run.r;
@@ -530,21 +569,29 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) k_policy_rows(const __g
             cut += double(clipped ? w : 0.f);
         }
         if (GRAD) {
-            const GradOf<T> grad(z, g, sl, r.token, u, R, s, c, far);
+            const GradOf<T> grad(z, g, sl, V, r.token, u, R, s, c, far);
             grad.ends(sl, tid);
-            const uint32_t from = in.freed;
-            for (int k = 0; k < chunks; ++k) {
+            const bool plain = grad.plain();
+            uint4* o = reinterpret_cast<uint4*>(g + sl.body) + first + lane;
+            for (int k = 0, left = sl.hi - first; k < chunks; ++k, left -= in.kStride, o += in.kStride) {
                 uint4 q[4];
-                if (!fits) in.wait(from + k);
-                in.read(from + k, q);
-                const int v0 = first + k * in.kStride + lane;
+                if (!fits) in.wait(in.at_);
+                in.read(in.at_, q);
+                const int v0 = sl.hi - left + lane;
+                if (plain && left >= kChunk) {
 #pragma unroll
-                for (int v = 0; v < 4; ++v)
-                    if (v0 + 32 * v < sl.hi) grad.vec(sl.body, v0 + 32 * v, q[v]);
+                    for (int v = 0; v < 4; ++v) grad.vec_plain(o + 32 * v, q[v]);
+                    if (unsigned(grad.token_vec - v0) < 128u && ((grad.token_vec - v0) & 31) == 0) grad.one(grad.token, za);
+                } else {
+#pragma unroll
+                    for (int v = 0; v < 4; ++v)
+                        if (lane + 32 * v < left) grad.vec(sl.body, v0 + 32 * v, q[v]);
+                }
                 in.release();
             }
         }
     }
+    let_next_start();
     if (rank == 0 && tid == 0) {
         double* p = partials_of(a) + 3 * unit;
         p[0] = loss;
@@ -560,6 +607,7 @@ __global__ void __launch_bounds__(1024) k_policy_plan(const __grid_constant__ cr
     __shared__ int before[32];
     const int n = int(a.batch * a.steps), steps = int(a.steps), tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
     const int per = (n + 1023) / 1024;
+    let_next_start();
     const int lo = int(tmin<int64_t>(n, int64_t(tid) * per)), hi = int(tmin<int64_t>(n, int64_t(lo) + per));
     double v = 0;
     int c = 0;
@@ -604,6 +652,7 @@ __global__ void __launch_bounds__(768) k_policy_sums(const __grid_constant__ crx
     __shared__ double red[24];
     const int w = threadIdx.x >> 5, i = w >> 3, lane = threadIdx.x & 31;   // eight warps per term
     double v = 0;
+    after_previous();
     for (int k = threadIdx.x & 255; k < units; k += 256) v += partials_of(a)[3 * k + i];
     v = warp_sum(v);
     if (lane == 0) red[w] = v;
@@ -634,7 +683,7 @@ __global__ void __launch_bounds__(kRowThreads) k_policy_again(const __grid_const
                                          : static_cast<const int32_t*>(a.tokens.p)[at(a.tokens, b, t)];
         const float u = saved.x == 0.f ? 0.f : saved.x * f;   // a row that does not count stays 0 whatever the scale
         const Slice sl = slice_of<T>(z, a.vocab, int(item - row * C), C);
-        GradOf<T>(z, g, sl, token, u, saved.y, saved.z, c, saved.w != 0.f).slice(sl, threadIdx.x, kRowThreads);
+        GradOf<T>(z, g, sl, a.vocab, token, u, saved.y, saved.z, c, saved.w != 0.f).slice(sl, threadIdx.x, kRowThreads);
     }
 }
 
@@ -645,14 +694,26 @@ int fail(char* err, size_t errlen, int status, const std::string& msg) {
     return status;
 }
 
-// A row by one warp, where its ring holds one: no warp waits for another.
-bool warp_rows(int64_t n, int64_t V, int vec) { return V <= int64_t(kSlots) * kChunk * vec && n >= kRowGrid; }
+// A row that does not fit the rings is read a second time for its gradient, out of L2 as long as the
+// rows that are being worked on at once are no more than this (of 126 MB; the gradients pass through
+// it too).  2143 MB of 4096 x 152k bf16 rows, a quarter masked: 0.39 ms with 45 MB of rows at once,
+// 0.48 with 90, 0.44 with 180; 2048 x 152k fp32 0.46, 0.57, 0.60.
+constexpr int64_t kRowsAtOnce = int64_t(48) << 20;
 
-// CTAs per row: enough for the rings to hold one (with a gradient: its logits are then read once), and
-// as many as the rows leave room for while a slice keeps two chunks.
+// A row by one warp, where nothing waits for another warp: rows that its ring holds, and longer ones
+// when there are enough of them to go round twice (16384 x 8192 bf16: 0.15 ms by CTAs of four warps).
+bool warp_rows(int64_t n, int64_t V, int vec) {
+    const int64_t bytes = V / vec * 16;
+    return bytes <= int64_t(kSlots) * kChunk * 16 ? n >= kRowGrid : n >= 2 * kMaxUnits && bytes * kMaxUnits <= kRowsAtOnce;
+}
+
+// CTAs per row: enough to keep the rows at once in L2 (with a gradient), and as many as the rows leave
+// room for while a slice keeps two chunks per warp.
 int cluster_for(int64_t n, int64_t V, int vec, bool grad) {
+    const int64_t bytes = V / vec * 16;
     int C = 1;
-    while (C < kMaxCluster && ((grad && V > int64_t(kRowWarps) * kSlots * kChunk * vec * C) || (n * C * 2 <= kRowGrid && V >= int64_t(kChunk) * vec * 4 * C)))
+    while (C < kMaxCluster && ((grad && std::min<int64_t>(n, kRowGrid / C) * bytes > kRowsAtOnce) ||
+                               (n * C * 2 <= kRowGrid && bytes >= int64_t(kChunk) * 16 * 4 * C)))
         C *= 2;
     return C;
 }
@@ -665,7 +726,7 @@ cudaError_t launch_as(const crx_policy_args& a, double inv_denom, int C, int64_t
     cfg.gridDim = dim3(kRowGrid / C * C);
     cfg.dynamicSmemBytes = kRingBytes;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = unsigned(C);
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
@@ -690,6 +751,11 @@ cudaError_t launch_as(const crx_policy_args& a, double inv_denom, int C, int64_t
     const int grid = int(std::min<int64_t>(most, clusters));
     *units = WARP ? grid * kRowWarps : grid;
     cfg.gridDim = dim3(unsigned(grid * C));
+    if (a.mask.p) {   // directly behind the plan
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.numAttrs = 2;
+    }
     return cudaLaunchKernelEx(&cfg, kernel, a, inv_denom, int(a.mask.p != nullptr), C);
 }
 
@@ -763,10 +829,7 @@ int crx_policy_loss(const crx_policy_args* args, void* stream, char* err, size_t
             else if (a.dtype == CRX_FP16) e = grad ? launch_rows<__half, true>(a, inv_denom, &units, st) : launch_rows<__half, false>(a, inv_denom, &units, st);
             else e = grad ? launch_rows<float, true>(a, inv_denom, &units, st) : launch_rows<float, false>(a, inv_denom, &units, st);
         }
-        if (e == cudaSuccess) {
-            k_policy_sums<<<1, 768, 0, st>>>(a, inv_denom, units);
-            e = cudaGetLastError();
-        }
+        if (e == cudaSuccess) e = launch_behind(k_policy_sums, 1, 768, st, a, inv_denom, units);
         return e == cudaSuccess ? CRX_OK : fail(err, errlen, CRX_CUDA_ERROR, std::string("crx_policy_loss: ") + cudaGetErrorString(e));
     } catch (const std::exception& ex) {
         return fail(err, errlen, CRX_NO_MEMORY, std::string("crx_policy_loss: ") + ex.what());
