@@ -269,33 +269,39 @@ struct StepRates {
     bool skip;   // the norm is not finite: masters and moments stay as they are
 };
 
-// Root and reciprocal to 1 ulp each: the exact ones took the step of 0.93e9 parameters from 3.81 to
-// 4.87 ms, for two roundings that are 2^-24 of an update that is itself a small part of the master.
+// Root and reciprocal to 1 ulp each, values below 2^-126 taken as 0: next to an eps of kTinyEps or
+// more such a root (2^-63) is nothing.  Back to back, the step of 0.93e9 parameters takes 3.80 ms with
+// these, 4.14 with the ones that mind such values, 4.87 with the exactly rounded ones; their error is
+// 2^-22 of an update that is itself a small part of the master.
 __device__ __forceinline__ float sqrt_fast(float x) {
     float y;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 __device__ __forceinline__ float rcp_fast(float x) {
     float y;
-    asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+constexpr double kTinyEps = 1e-12;
 
+// TINY: the eps is less than kTinyEps, so root and quotient are the exactly rounded ones.
+template <bool TINY>
 __device__ __forceinline__ void adamw_one(const StepRates& r, float g, float& p, float& m, float& v) {
     g *= r.c;
     m = fmaf(r.b1, m, r.a1 * g);
     v = fmaf(r.b2, v, r.a2 * g * g);
-    const float den = sqrt_fast(v * r.inv_bias2) + r.eps;
-    p -= fmaf(r.decay, p, (r.rate * m) * rcp_fast(den));   // both terms first: p is rounded once
+    const float x = v * r.inv_bias2, y = r.rate * m;
+    const float up = TINY ? y / (sqrtf(x) + r.eps) : y * rcp_fast(sqrt_fast(x) + r.eps);
+    p -= fmaf(r.decay, p, up);   // both terms first: p is rounded once
 }
 
-template <class T>
+template <class T, bool TINY>
 __device__ __forceinline__ void step_scalar(const StepEntry& e, const StepRates& r, int64_t i) {
     float p = e.p[i];
     if (!r.skip) {
         float m = e.m[i], v = e.v[i];
-        adamw_one(r, to_f(static_cast<const T*>(e.g)[i]), p, m, v);
+        adamw_one<TINY>(r, to_f(static_cast<const T*>(e.g)[i]), p, m, v);
         e.p[i] = p;
         e.m[i] = m;
         e.v[i] = v;
@@ -316,15 +322,15 @@ __device__ __forceinline__ void load8_g(const T* s, float* x) { Vec<T>::get(*rei
 template <>
 __device__ __forceinline__ void load8_g<float>(const float* s, float* x) { load8(s, x); }
 
-template <class T>
+template <class T, bool TINY>
 __device__ __forceinline__ void tile_step(const StepEntry& e, const StepRates& r, int64_t k) {
     const int tid = threadIdx.x;
     if (e.head < 0) {   // no common alignment
         const int64_t base = k * kStepTile, end = tmin<int64_t>(e.numel, base + kStepTile);
-        for (int64_t i = base + tid; i < end; i += kThreads) step_scalar<T>(e, r, i);
+        for (int64_t i = base + tid; i < end; i += kThreads) step_scalar<T, TINY>(e, r, i);
         return;
     }
-    if (k == 0 && tid < tmin<int64_t>(e.head, e.numel)) step_scalar<T>(e, r, tid);
+    if (k == 0 && tid < tmin<int64_t>(e.head, e.numel)) step_scalar<T, TINY>(e, r, tid);
     const int64_t i = e.head + k * kStepTile + tid * 8;
     if (i + 8 <= e.numel) {
         float g[8], p[8], m[8], v[8];
@@ -334,18 +340,18 @@ __device__ __forceinline__ void tile_step(const StepEntry& e, const StepRates& r
             load8(e.m + i, m);
             load8(e.v + i, v);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) adamw_one(r, g[j], p[j], m[j], v[j]);
+            for (int j = 0; j < 8; ++j) adamw_one<TINY>(r, g[j], p[j], m[j], v[j]);
             store8(e.p + i, p);
             store8(e.m + i, m);
             store8(e.v + i, v);
         }
         if (e.w) *reinterpret_cast<uint4*>(e.w + i) = Vec<__nv_bfloat16>::put(p);
     } else {
-        for (int64_t j = i; j < e.numel; ++j) step_scalar<T>(e, r, j);
+        for (int64_t j = i; j < e.numel; ++j) step_scalar<T, TINY>(e, r, j);
     }
 }
 
-template <class Tab>
+template <bool TINY, class Tab>
 __global__ void __launch_bounds__(kThreads) k_adamw(const __grid_constant__ Tab t, const __grid_constant__ StepHyper h) {
     StepRates r;
     r.skip = false;
@@ -372,9 +378,9 @@ __global__ void __launch_bounds__(kThreads) k_adamw(const __grid_constant__ Tab 
     r.eps = h.eps;
     const StepEntry& e = t.e[tensor_of(t, blockIdx.x)];
     const int64_t k = blockIdx.x - e.tile;
-    if (e.dtype == CRX_FP32) tile_step<float>(e, r, k);
-    else if (e.dtype == CRX_BF16) tile_step<__nv_bfloat16>(e, r, k);
-    else tile_step<__half>(e, r, k);
+    if (e.dtype == CRX_FP32) tile_step<float, TINY>(e, r, k);
+    else if (e.dtype == CRX_BF16) tile_step<__nv_bfloat16, TINY>(e, r, k);
+    else tile_step<__half, TINY>(e, r, k);
 }
 
 // ------------------------------------------------------------------ host
@@ -647,7 +653,8 @@ int crx_adamw_step(int32_t n, float* const* master, const void* const* grads, co
                 return uint32_t(std::max<int64_t>(1, (body + kStepTile - 1) / kStepTile));
             },
             [&](const auto& t) {
-                k_adamw<<<t.tiles, kThreads, 0, st>>>(t, h);
+                if (args->eps < kTinyEps) k_adamw<true><<<t.tiles, kThreads, 0, st>>>(t, h);
+                else k_adamw<false><<<t.tiles, kThreads, 0, st>>>(t, h);
                 return cudaGetLastError();
             });
         return e == cudaSuccess ? CRX_OK : cuda_fail(err, errlen, "crx_adamw_step", e);

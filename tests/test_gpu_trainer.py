@@ -261,6 +261,25 @@ def test_adamw_first_step_from_zero_moments(crx, b1, b2):
         near(d["a"], x, t)
 
 
+@pytest.mark.parametrize("eps", [1e-30, 1e-15, 9e-13, 1e-12, 1e-6])
+def test_adamw_of_tiny_gradients(crx, eps):
+    """Second moments near and below the smallest normal number, next to an eps of any size."""
+    g = torch.randn(20000, generator=gen(3)) * torch.logspace(-23, -15, 20000)
+    p, z = torch.zeros(20000), torch.zeros(20000)
+    dev = [{"a": t.cuda()} for t in (p, z, z)]
+    crx.adamw_step(dev[0], {"a": g.cuda()}, dev[1], dev[2], lr=1e-3, step=1, eps=eps)
+    want, tol = ref.adamw(p, g, z, z, lr=1e-3, step=1, b1=0.9, b2=0.999, eps=eps, wd=0.0)
+    # below 2^-126 the root may count as 0: at most 2^-63 / eps of the update, where eps is 1e-12 or more;
+    # and v is a multiple of 2^-149, so its root is known to half of that over the root
+    v = want[2]
+    loose = want[0].abs() * (2.0 ** -63 / eps if eps >= 1e-12 else 0.0)
+    den = (v / (1 - 0.999)).sqrt()
+    steps = want[0].abs() * 2.0 * (2.0 ** -149 / (1 - 0.999)) / (den * (den + eps)).clamp(min=1e-60)
+    fine = steps < 0.1 * want[0].abs()   # (elsewhere v is a few of its steps and says nothing)
+    near(dev[0]["a"].cpu()[fine], want[0][fine], (tol[0] + loose + steps)[fine])
+    near(dev[2]["a"], v, tol[2])
+
+
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 def test_adamw_leaves_the_state_when_the_norm_is_not_finite(crx, bad):
     cpu, gpu = gradients([4001], torch.float32, 12)
