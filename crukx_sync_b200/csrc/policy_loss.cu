@@ -357,11 +357,12 @@ struct GradOf {
 
 // What a row needs besides its logits.
 struct RowIn {
-    int64_t row, at, grad_at, token;
+    uint32_t row;
+    int64_t at, grad_at, token;
     float w, advantage, old, ref;
 };
-__device__ __forceinline__ RowIn row_in(const crx_policy_args& a, int64_t row) {
-    const int64_t b = row / a.steps, t = row - b * a.steps;
+__device__ __forceinline__ RowIn row_in(const crx_policy_args& a, uint32_t row) {
+    const uint32_t b = row / uint32_t(a.steps), t = row - b * uint32_t(a.steps);
     RowIn r;
     r.row = row;
     r.at = at(a.logits, b, t);
@@ -380,6 +381,9 @@ __device__ __forceinline__ double warp_sum(double v) {
     return v;
 }
 
+// The row at place i of the plan's order (of `n` places).
+__device__ __forceinline__ uint32_t row_at(const int32_t* order, uint32_t i, uint32_t n) { return !order ? i : i < n ? uint32_t(order[i]) : 0; }
+
 // A place in a warp's ring, and the phase of its barrier that says that the chunk is here.
 struct Place {
     uint32_t slot = 0, phase = 0;
@@ -397,7 +401,8 @@ template <class T, bool GRAD, bool WARP>
 struct Stream {
     const crx_policy_args& a;
     uint32_t ring, bars;       // shared addresses: kSlots chunks, kSlots barriers
-    int64_t i, step, n;        // place of the row being issued among those that count, the unit's stride, their number
+    uint32_t i, step, n;       // place of the row being issued among those that count, the unit's stride, their number
+    uint32_t row_after;        // the row at the place after that, loaded ahead
     const int32_t* order;
     int rank, C;
     const char* from;          // its next vector
@@ -407,9 +412,9 @@ struct Stream {
 
     static constexpr int kStride = WARP ? kChunk : kChunk * kRowWarps;
 
-    __device__ __forceinline__ Stream(const crx_policy_args& a, char* mem, uint64_t* bars_, int64_t i, int64_t step, int64_t n,
+    __device__ __forceinline__ Stream(const crx_policy_args& a, char* mem, uint64_t* bars_, uint32_t i, uint32_t step, uint32_t n,
                                       const int32_t* order, int rank, int C)
-        : a(a), i(i), step(step), n(n), order(order), rank(rank), C(C) {
+        : a(a), i(i), step(step), n(n), row_after(row_at(order, i, n)), order(order), rank(rank), C(C) {
         const int warp = threadIdx.x >> 5;
         ring = smem_of(mem) + uint32_t(warp) * (kSlots * kChunk * 16);
         bars = smem_of(bars_ + warp * kSlots);
@@ -425,7 +430,8 @@ struct Stream {
     // goes on to the next row that has a part for this warp
     __device__ __forceinline__ void open() {
         for (; i < n; i += step) {
-            const int64_t row = order ? order[i] : i, b = row / a.steps, t = row - b * a.steps;
+            const uint32_t row = row_after, b = row / uint32_t(a.steps), t = row - b * uint32_t(a.steps);
+            row_after = row_at(order, i + step, n);
             const T* z = static_cast<const T*>(a.logits.p) + at(a.logits, b, t);
             const Slice sl = slice_of<T>(z, a.vocab, rank, C);
             span = left = sl.hi - first(sl);
@@ -481,9 +487,10 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) k_policy_rows(const __g
     __shared__ Shared sh;
     const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, lane = threadIdx.x & 31, threads = WARP ? 32 : kRowThreads;
     const int rank = WARP ? 0 : int(blockIdx.x) % C;
-    const int64_t n = a.batch * a.steps, V = a.vocab;
-    const int64_t unit = WARP ? int64_t(blockIdx.x) * kRowWarps + (threadIdx.x >> 5) : blockIdx.x / C;
-    const int64_t units = WARP ? int64_t(gridDim.x) * kRowWarps : gridDim.x / C;
+    const int64_t V = a.vocab;
+    const uint32_t n = uint32_t(a.batch * a.steps);
+    const uint32_t unit = WARP ? blockIdx.x * kRowWarps + (threadIdx.x >> 5) : blockIdx.x / C;
+    const uint32_t units = WARP ? gridDim.x * kRowWarps : gridDim.x / C;
     if (threadIdx.x < kRowWarps * kSlots + 2)
         asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_of(threadIdx.x < kRowWarps * kSlots ? &bars[threadIdx.x] : &sh.came[threadIdx.x - kRowWarps * kSlots]))
                      : "memory");
@@ -494,21 +501,25 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) k_policy_rows(const __g
     const float c = float(1.4426950408889634 / double(a.temperature));
     const float inv_d = float(inv_denom < 0 ? plan_of(a)->inv_denom : inv_denom), inv_tau = 1.f / a.temperature;
     const int32_t* order = planned ? order_of(a) : nullptr;
-    const int64_t counted = planned ? plan_of(a)->counted : n;
+    const uint32_t counted = planned ? uint32_t(plan_of(a)->counted) : n;
     double loss = 0, kl = 0, cut = 0;
     uint32_t nth = 0;   // of the unit's rows that count
     Stream<T, GRAD, WARP> in(a, ring, bars, unit, units, counted, order, rank, C);
     RowIn next;
-    if (unit < n) next = row_in(a, order ? order[unit] : unit);
-    for (int64_t i = unit; i < n; i += units) {
+    if (unit < n) next = row_in(a, row_at(order, unit, n));
+    uint32_t row_after = row_at(order, unit + units, n);
+    for (uint32_t i = unit; i < n; i += units) {
         const RowIn r = next;
         const float w = r.w;
-        const int64_t row = r.row;
+        const uint32_t row = r.row;
         const T* z = static_cast<const T*>(a.logits.p) + r.at;
         T* g = GRAD ? static_cast<T*>(const_cast<void*>(a.grad.p)) + r.grad_at : nullptr;
         const Slice sl = slice_of<T>(z, V, rank, C);
         const float za = i < counted && r.token >= 0 && r.token < V ? to_f(z[r.token]) : NAN;
-        if (i + units < n) next = row_in(a, order ? order[i + units] : i + units);   // (its latency passes under this row)
+        if (i + units < n) {   // what the next row needs, and the number of the one after it: they arrive under this row
+            next = row_in(a, row_after);
+            row_after = row_at(order, i + 2 * units, n);
+        }
         if (i >= counted) {
             if (GRAD) GradOf<T>(z, g, sl, V, -1, 0.f, 0.f, 1.f, c, false).slice(sl, tid, threads);
             if (rank == 0 && tid == 0) {
