@@ -117,6 +117,23 @@ def load():
     return _lib
 
 
+_glue_module = None
+
+
+def glue():
+    """The torch side of trainer.py's calls (csrc/glue/torch_glue.cpp, built in-tree beside the library)."""
+    global _glue_module
+    if _glue_module is None:
+        load()
+        try:
+            from . import _glue
+        except ImportError as exc:
+            raise ImportError(f"{os.path.join(_HERE, '_glue.so')} is missing or does not load: build it first "
+                              f"(python -m crukx_sync_b200.build, or __graft_entry__.build()): {exc}") from exc
+        _glue_module = _glue
+    return _glue_module
+
+
 _ctx = {}
 
 

@@ -1,4 +1,5 @@
-"""Build the in-tree CUDA library ``crukx_sync_b200/libcrukx_b200.so`` for sm_100a with nvcc.
+"""Build the in-tree CUDA library ``crukx_sync_b200/libcrukx_b200.so`` for sm_100a with nvcc, and the
+torch side of trainer.py's calls, ``crukx_sync_b200/_glue.so``, with g++.
 
     python -m crukx_sync_b200.build [--force] [--verbose]
 
@@ -10,16 +11,20 @@ from __future__ import annotations
 
 import concurrent.futures
 import glob
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libcrukx_b200.so")
+GLUE_SRC = os.path.join(CSRC, "glue", "torch_glue.cpp")
+GLUE = os.path.join(HERE, "_glue.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O3", "-I", os.path.join(ROOT, "include"),
          "--expt-relaxed-constexpr"]
@@ -39,6 +44,17 @@ def cxx() -> str:
 def _headers():
     return glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(CSRC, "*.cuh")) + \
         glob.glob(os.path.join(ROOT, "include", "*.h"))
+
+
+def glue_command(out: str) -> list[str]:
+    torch = os.path.dirname(importlib.util.find_spec("torch").origin)   # (found, not imported: that takes a while)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
+    include = [os.path.join(torch, "include"), os.path.join(torch, "include", "torch", "csrc", "api", "include"),
+               sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    return [cxx(), "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_glue", "-DTORCH_API_INCLUDE_EXTENSION_H",
+            *[x for d in include for x in ("-I", d)], GLUE_SRC, "-o", out, "-L", HERE, "-l:libcrukx_b200.so",
+            "-L", os.path.join(torch, "lib"), "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
+            "-Wl,-rpath,$ORIGIN"]
 
 
 def build(force: bool = False, verbose: bool = False, extra: list[str] | None = None) -> str:
@@ -64,7 +80,7 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
             print(" ".join(cmd), flush=True)
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
-            raise RuntimeError(f"nvcc failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+            raise RuntimeError(f"compiler failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
         if verbose and (r.stdout or r.stderr):
             print(r.stdout + r.stderr, flush=True)
 
@@ -74,6 +90,11 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
         tmp = LIB + ".tmp"
         run([cc, *ARCH, "-shared", "-o", tmp, *objs, "-lcudart"])
         os.replace(tmp, LIB)
+    header = os.path.join(ROOT, "include", "crukx_b200.h")
+    if force or not os.path.exists(GLUE) or os.path.getmtime(GLUE) < max(os.path.getmtime(GLUE_SRC), os.path.getmtime(header)):
+        tmp = GLUE + ".tmp"
+        run(glue_command(tmp))
+        os.replace(tmp, GLUE)
     return LIB
 
 

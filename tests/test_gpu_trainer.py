@@ -593,6 +593,27 @@ def test_backward_twice(crx):
         torch.autograd.grad(out.loss, z)
 
 
+def test_a_gradient_of_the_gradient_is_refused(crx):
+    d = batch(1, 2, 50, torch.float32, 19)
+    z = d["logits"].cuda().requires_grad_()
+    out = crx.policy_loss(z, dev(d["tokens"]), dev(d["adv"]))
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(out.loss, z, create_graph=True)
+
+
+def test_inference_tensors_are_not_written(crx):
+    with torch.inference_mode():
+        t = torch.ones(8, device="cuda")
+        near(crx.grad_norm({"t": t}), math.sqrt(8), math.sqrt(8) * ref.NORM)
+        crx.clip_grads({"t": t}, 1.0)
+    near(t.clone(), torch.full((8,), 1 / math.sqrt(8)), 1e-6)
+    before = t.clone()
+    near(crx.grad_norm({"t": t}), 1.0, 1e-6)
+    with pytest.raises(ValueError, match="inference"):
+        crx.clip_grads({"t": t}, 0.5)
+    assert torch.equal(t.clone(), before)
+
+
 def test_logits_changed_before_backward_are_noticed(crx):
     d = batch(1, 2, 50, torch.float32, 19)
     z = d["logits"].cuda().requires_grad_()
