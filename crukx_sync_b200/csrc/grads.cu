@@ -64,15 +64,15 @@ struct StepEntry {
     int16_t dtype;
     int16_t head;       // elements before the first place where every pointer is 16-byte aligned; -1: none
 };
-// The table is a kernel parameter, at most 32764 bytes of them.  The small one keeps a call over a
-// few tensors from copying 31 KB of parameters per launch.
+// The table is a kernel parameter, at most 32764 bytes of them.  A launch copies all of it (the norm of
+// 112 tensors took 23 us of the host with a table of 960), so there are several sizes.
 template <class E, int N>
 struct Table {
     E e[N];
     int32_t n;
     uint32_t tiles;
 };
-constexpr int kSmall = 40, kGradLarge = 960, kStepLarge = 500;
+constexpr int kSmall = 40, kMedium = 160, kGradLarge = 960, kStepLarge = 500;
 static_assert(sizeof(Table<GradEntry, kGradLarge>) < 32000 && sizeof(Table<StepEntry, kStepLarge>) < 32300, "parameter space");
 
 template <class T>
@@ -404,7 +404,8 @@ struct Range {
 
 // Two tensors of which at least one is written may not share memory (a race otherwise).
 bool overlap(std::vector<Range>& r, int32_t* a, int32_t* b) {
-    std::sort(r.begin(), r.end(), [](const Range& x, const Range& y) { return x.lo < y.lo; });
+    const auto below = [](const Range& x, const Range& y) { return x.lo < y.lo; };
+    if (!std::is_sorted(r.begin(), r.end(), below)) std::sort(r.begin(), r.end(), below);
     const Range* any = nullptr;       // the range so far that reaches furthest
     const Range* written = nullptr;   // and the written one
     for (const Range& x : r) {
@@ -464,8 +465,9 @@ cudaError_t all_tables(int32_t n, const int64_t* numel, Fill fill, Launch launch
     int32_t filled = 0;
     for (int32_t i = 0; i < n; ++i) filled += numel[i] != 0;
     for (int32_t at = 0; at < n;) {
-        const cudaError_t e = filled <= kSmall ? each_table<E, kSmall>(n, numel, &at, fill, launch)
-                                               : each_table<E, Large>(n, numel, &at, fill, launch);
+        const cudaError_t e = filled <= kSmall    ? each_table<E, kSmall>(n, numel, &at, fill, launch)
+                              : filled <= kMedium ? each_table<E, kMedium>(n, numel, &at, fill, launch)
+                                                  : each_table<E, Large>(n, numel, &at, fill, launch);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
@@ -539,9 +541,12 @@ int crx_clip_grads(int32_t n, const void* const* grads, void* const* out, const 
             const int64_t bytes = numel[i] * elem_size(dtypes[i]);
             if (!out[i] || reinterpret_cast<uintptr_t>(out[i]) % elem_size(dtypes[i]))
                 return fail(err, errlen, CRX_BAD_ARGUMENT, "crx_clip_grads: null or misaligned output " + std::to_string(i));
-            const uintptr_t g = reinterpret_cast<uintptr_t>(grads[i]), o = reinterpret_cast<uintptr_t>(out[i]);
-            if (g != o) r.push_back(Range{g, g + uintptr_t(bytes), false, i});
+            const uintptr_t o = reinterpret_cast<uintptr_t>(out[i]);
             r.push_back(Range{o, o + uintptr_t(bytes), true, i});
+        }
+        for (int32_t i = 0; i < n; ++i) {
+            const uintptr_t g = reinterpret_cast<uintptr_t>(grads[i]);
+            if (numel[i] && out[i] != grads[i]) r.push_back(Range{g, g + uintptr_t(numel[i]) * elem_size(dtypes[i]), false, i});
         }
         int32_t a, b;
         if (overlap(r, &a, &b))
