@@ -94,6 +94,8 @@ struct Set {
     }
 };
 
+float narrow(double x) { return static_cast<float>(std::min(x, 3.0e38)); }   // of a limit: what fp32 holds of it
+
 at::TensorOptions on(int dev, at::ScalarType t) { return at::TensorOptions().device(at::kCUDA, static_cast<c10::DeviceIndex>(dev)).dtype(t); }
 void* stream_of(int dev) { return c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(dev)).stream(); }
 
@@ -143,7 +145,7 @@ py::object clip_grads(const py::dict& grads, double max_norm, const c10::optiona
         ws = at::empty({bytes}, on(g.dev, at::kByte));
     }
     char err[512] = "";
-    const int st = crx_clip_grads(n, g.ptr.data(), to.ptr.data(), g.code.data(), g.numel.data(), static_cast<float>(max_norm), norm_in,
+    const int st = crx_clip_grads(n, g.ptr.data(), to.ptr.data(), g.code.data(), g.numel.data(), narrow(max_norm), norm_in,
                                   norm ? nullptr : ws.data_ptr(), bytes, norm ? nullptr : result.data_ptr<float>(), stream_of(g.dev), err,
                                   sizeof err);
     if (st != CRX_OK) fail(st, err);
@@ -170,7 +172,7 @@ bool adamw_step(const py::dict& masters, const py::dict& grads, const py::dict& 
     a.eps = eps;
     a.weight_decay = weight_decay;
     a.step = step;
-    a.max_norm = static_cast<float>(max_norm);
+    a.max_norm = narrow(max_norm);
     const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(g.dev));
     char err[512] = "";
     const int st = crx_adamw_step(static_cast<int32_t>(g.t.size()), reinterpret_cast<float* const*>(p.ptr.data()), g.ptr.data(), g.code.data(),
@@ -330,8 +332,8 @@ py::object policy_loss(const at::Tensor& logits, const at::Tensor& tokens, const
     if (ref_logp && (ref_logp->scalar_type() != at::kFloat || !rows(*ref_logp, tokens, false, &a.ref_logp))) return py::none();
     if (mask && ((mask->scalar_type() != at::kFloat && mask->scalar_type() != at::kBool) || !rows(*mask, tokens, true, &a.mask))) return py::none();
     a.denom = denom;
-    a.clip_low = static_cast<float>(clip_low);
-    a.clip_high = static_cast<float>(clip_high);
+    a.clip_low = narrow(clip_low);
+    a.clip_high = narrow(clip_high);
     a.kl_coef = static_cast<float>(kl_coef);
     a.temperature = static_cast<float>(temperature);
     a.dtype = type_code(logits.scalar_type());

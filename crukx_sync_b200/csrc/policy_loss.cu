@@ -569,13 +569,13 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) k_policy_rows(const __g
         if (a.ref_logp.p) {
             const float x = r.ref - logp, e = expm1f(x);
             k = e - x;
-            dl -= a.kl_coef * e;
+            if (a.kl_coef != 0.f) dl -= a.kl_coef * e;   // (a k that is only reported may overflow)
         }
         const float u = w * inv_d * dl * inv_tau;
         if (rank == 0 && tid == 0) {
             a.logp[row] = logp;
             saved_of(a)[row] = make_float4(u, R, s, far ? 1.f : 0.f);
-            loss += double(w * (a.kl_coef * k - gain));
+            loss += double(w * ((a.kl_coef != 0.f ? a.kl_coef * k : 0.f) - gain));
             kl += double(w * k);
             cut += double(clipped ? w : 0.f);
         }
@@ -788,7 +788,7 @@ cudaError_t launch_again(const crx_policy_args& a, const float* scale, int unles
 int check(const char* who, const crx_policy_args* a, char* err, size_t errlen) {
     const auto bad = [&](const char* what) { return fail(err, errlen, CRX_BAD_ARGUMENT, std::string(who) + ": " + what); };
     if (!a) return bad("null arguments");
-    if (a->batch < 0 || a->steps < 0 || a->vocab < 1 || a->vocab > (int64_t(1) << 31) || a->batch > (int64_t(1) << 31) || a->steps > (int64_t(1) << 31) ||
+    if (a->batch < 0 || a->steps < 0 || a->vocab < 1 || a->vocab > (int64_t(1) << 30) || a->batch > (int64_t(1) << 31) || a->steps > (int64_t(1) << 31) ||
         (a->batch && a->steps >= (int64_t(1) << 31) / a->batch))
         return bad("size out of range");
     if (a->dtype != CRX_BF16 && a->dtype != CRX_FP16 && a->dtype != CRX_FP32) return bad("unknown type");
@@ -798,8 +798,8 @@ int check(const char* who, const crx_policy_args* a, char* err, size_t errlen) {
         if (!a->logits.p || !a->tokens.p || !a->advantages.p || !a->logp) return bad("null pointer");
         if (reinterpret_cast<uintptr_t>(a->logits.p) % es || reinterpret_cast<uintptr_t>(a->grad.p) % es) return bad("misaligned logits or gradient");
     }
-    if (!(a->temperature > 0.f) || !(a->clip_low >= 0.f) || !(a->clip_high >= 0.f) || !(a->denom >= 0) || !std::isfinite(a->temperature))
-        return fail(err, errlen, CRX_VALUE_ERROR, "temperature must be positive and finite, clip bounds and denom not negative");
+    if (!(a->temperature >= 1e-30f) || !(a->clip_low >= 0.f) || !(a->clip_high >= 0.f) || !(a->denom >= 0) || !std::isfinite(a->temperature))
+        return fail(err, errlen, CRX_VALUE_ERROR, "temperature must be at least 1e-30 and finite, clip bounds and denom not negative");
     return CRX_OK;
 }
 

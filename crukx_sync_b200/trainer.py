@@ -212,10 +212,10 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, advantages: torch.Te
     lo, hi = clip
     if not (lo >= 0 and hi >= 0):
         raise ValueError(f"clip bounds must not be negative, got {clip}")
-    if not 0 < temperature < math.inf:
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
-    if not math.isfinite(kl_coef):
-        raise ValueError(f"kl_coef must be finite, got {kl_coef}")
+    if not 1e-30 < temperature < math.inf:   # (1 / temperature is a number fp32 holds)
+        raise ValueError(f"temperature must be more than 1e-30 and finite, got {temperature}")
+    if not abs(kl_coef) < 1e30:
+        raise ValueError(f"kl_coef must be less than 1e30, got {kl_coef}")
     if kl_coef and ref_logp is None:
         raise ValueError("kl_coef needs ref_logp")
     if denom is not None and not denom > 0:

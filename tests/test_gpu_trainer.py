@@ -556,6 +556,36 @@ def test_zero_advantage_and_far_ratios(crx):
     assert torch.isfinite(out.loss) and not grad[0, :4].any()
 
 
+def test_a_reference_that_is_only_reported(crx):
+    """Without a coefficient the KL term may be anything: loss and gradient do not see it."""
+    d = batch(1, 4, 200, torch.float32, 16)
+    base, grad = run(crx, {**d, "ref": None})
+    d["ref"][0, 1] = 200.0
+    out, grad2 = run(crx, d)
+    assert torch.equal(out.loss, base.loss) and torch.equal(grad, grad2) and out.kl == math.inf
+
+
+@pytest.mark.parametrize("clip", [(0.0, 0.0), (5.0, math.inf), (0.2, 1e300)])
+def test_clip_bounds_of_any_size(crx, clip):
+    d = batch(2, 20, 300, torch.float32, 22, with_ref=False)
+    d["old"] += 0.01   # no ratio of exactly 1
+    verify(crx, d, clip=clip)
+
+
+def test_dicts_in_different_orders(crx):
+    cpu, gpu = gradients([100, 33, 7000], torch.bfloat16, 15)
+    host, dev = state_of(cpu)
+    turned = [dict(reversed(list(x.items()))) for x in dev]
+    w = {k: torch.zeros(t.numel(), dtype=torch.bfloat16, device="cuda") for k, t in sorted(cpu.items(), reverse=True)}
+    crx.adamw_step(turned[0], gpu, dev[1], turned[2], w, **step_args(3))
+    check_step(cpu, host, dev, w, 3)
+    out = {k: torch.zeros_like(t) for k, t in reversed(list(gpu.items()))}
+    crx.clip_grads(gpu, 1.0, out=out)
+    n = ref.norm(cpu.values())
+    for k in cpu:
+        near(out[k], *ref.clip(cpu[k], ref.coef(n, 1.0)), k)
+
+
 def test_empty_batches(crx):
     for shape in [(0,), (0, 4), (3, 0)]:
         z = torch.zeros(*shape, 10, device="cuda", requires_grad=True)

@@ -89,7 +89,7 @@ def test_loss_arguments_that_are_refused():
                       (dict(ref_logp=fake(3, 2)), "ref_logp"), (dict(mask=fake(2, 3, dtype=torch.int64)), "mask"), (dict(mask=fake(3)), "mask"),
                       (dict(adv=torch.zeros(2, 1)), "one device"), (dict(tok=torch.zeros(2, 3, dtype=torch.int64)), "one device"),
                       (dict(clip=(-0.1, 0.2)), "clip"), (dict(clip=(0.1, math.nan)), "clip"), (dict(temperature=0.0), "temperature"),
-                      (dict(temperature=math.inf), "temperature"), (dict(kl_coef=0.1), "ref_logp"), (dict(kl_coef=math.nan), "kl_coef"),
+                      (dict(temperature=math.inf), "temperature"), (dict(temperature=1e-38), "temperature"), (dict(kl_coef=0.1), "ref_logp"), (dict(kl_coef=math.nan), "kl_coef"), (dict(kl_coef=math.inf, ref_logp=fake(2, 3)), "kl_coef"),
                       (dict(denom=0.0), "denom"), (dict(denom=-1.0), "denom")]:
         with pytest.raises(ValueError, match=match):
             call(**kw)
@@ -154,7 +154,7 @@ def test_c_entry_points_refuse(lib):
     for kw, status in [(dict(batch=-1), 5), (dict(steps=-1), 5), (dict(vocab=0), 5), (dict(batch=1 << 30, steps=1 << 30), 5), (dict(logits=0), 5),
                        (dict(logits=4097), 5), (dict(tokens=0), 5), (dict(adv=0), 5), (dict(logp=0), 5), (dict(out=0), 5), (dict(stats=0), 5),
                        (dict(rows=0), 5), (dict(rows=4104), 5), (dict(dtype=3), 5), (dict(denom=-1.0), 1), (dict(lo=-0.5), 1), (dict(lo=math.nan), 1),
-                       (dict(tau=0.0), 1), (dict(tau=math.inf), 1)]:
+                       (dict(tau=0.0), 1), (dict(tau=math.inf), 1), (dict(tau=1e-38), 1), (dict(vocab=1 << 31), 5)]:
         assert loss(**kw) == status and err.value, kw
     assert lib.crx_policy_loss(None, None, err, 512) == 5 and lib.crx_policy_backward(None, None, 0, None, err, 512) == 5
 

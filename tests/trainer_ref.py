@@ -69,7 +69,7 @@ def policy(logits, tokens, adv, *, old=None, ref=None, mask=None, clip=(0.2, 0.2
     logp = logq.gather(-1, at)[..., 0]
     r = torch.ones_like(logp) if old is None else (logp - old.double()).exp()
     cut = ((A > 0) & (r > 1 + clip[1])) | ((A < 0) & (r < 1 - clip[0]))
-    bound = torch.where(A > 0, 1 + clip[1], 1 - clip[0])
+    bound = torch.where(A > 0, torch.tensor(1.0 + clip[1], dtype=torch.float64), 1.0 - clip[0])
     gain = torch.where(A == 0, 0.0, torch.where(cut, bound, r) * A)
     x = torch.zeros_like(logp) if ref is None else ref.double() - logp
     k = torch.expm1(x) - x
