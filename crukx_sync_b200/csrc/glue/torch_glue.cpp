@@ -33,8 +33,14 @@ int32_t type_code(at::ScalarType t) { return t == at::kBFloat16 ? CRX_BF16 : t =
     throw std::runtime_error("crukx_sync_b200: status " + std::to_string(status) + ": " + err);
 }
 
+bool same_name(PyObject* a, PyObject* b) {
+    return a == b || (PyUnicode_CheckExact(a) && PyUnicode_CheckExact(b) && PyUnicode_GET_LENGTH(a) == PyUnicode_GET_LENGTH(b) &&
+                      PyUnicode_Compare(a, b) == 0);
+}
+
+// Tensors of one dict (which keeps them alive through the call).
 struct Set {
-    std::vector<at::Tensor> t;
+    std::vector<c10::TensorImpl*> t;
     std::vector<void*> ptr;
     std::vector<int64_t> numel;
     std::vector<int32_t> code;
@@ -42,15 +48,16 @@ struct Set {
 
     bool add(PyObject* v, int types) {
         if (!THPVariable_Check(v)) return false;
-        const at::Tensor& x = THPVariable_Unpack(v);
-        if (!(type_bit(x.scalar_type()) & types) || !x.is_cuda() || x.layout() != at::kStrided || !x.is_contiguous()) return false;
-        const int d = x.get_device();
+        c10::TensorImpl* x = THPVariable_Unpack(v).unsafeGetTensorImpl();
+        const at::ScalarType type = c10::typeMetaToScalarType(x->dtype());
+        if (!(type_bit(type) & types) || !x->is_cuda() || x->layout() != at::kStrided || !x->is_contiguous()) return false;
+        const int d = x->device().index();
         if (dev < 0) dev = d;
         if (d != dev) return false;
         t.push_back(x);
-        ptr.push_back(x.data_ptr());
-        numel.push_back(x.numel());
-        code.push_back(type_code(x.scalar_type()));
+        ptr.push_back(x->mutable_data());
+        numel.push_back(x->numel());
+        code.push_back(type_code(type));
         return true;
     }
     void room(size_t n) {
@@ -72,25 +79,29 @@ struct Set {
         if (d.size() != like.size()) return false;
         room(d.size());
         dev = of.dev;
-        PyObject *k, *v;
-        Py_ssize_t at = 0;
+        PyObject *k, *v, *k2, *x;
+        Py_ssize_t at = 0, at2 = 0;
+        bool alike = true;   // so far d has its names in the same order: no lookups
         while (PyDict_Next(like.ptr(), &at, &k, &v)) {
-            PyObject* x = PyDict_GetItemWithError(d.ptr(), k);
-            if (!x) {
-                if (PyErr_Occurred()) throw py::error_already_set();
-                return false;
+            alike = alike && PyDict_Next(d.ptr(), &at2, &k2, &x) && same_name(k, k2);
+            if (!alike) {
+                x = PyDict_GetItemWithError(d.ptr(), k);
+                if (!x) {
+                    if (PyErr_Occurred()) throw py::error_already_set();
+                    return false;
+                }
             }
             if (!add(x, types)) return false;
         }
         return numel == of.numel;
     }
     bool writable() const {
-        return c10::InferenceMode::is_enabled() || std::none_of(t.begin(), t.end(), [](const at::Tensor& x) { return x.is_inference(); });
+        return c10::InferenceMode::is_enabled() || std::none_of(t.begin(), t.end(), [](c10::TensorImpl* x) { return x->is_inference(); });
     }
     // written through raw pointers: the version moves as for any in-place write
     void written() const {
-        for (const at::Tensor& x : t)
-            if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
+        for (c10::TensorImpl* x : t)
+            if (!x->is_inference()) x->bump_version();
     }
 };
 
