@@ -14,7 +14,7 @@ import crukx_sync_b200 as crx
 from crukx_sync_b200 import _ext, trainer
 
 
-@pytest.fixture(scope="module")
+@pytest.fixture(scope="module", autouse=True)
 def lib():
     from crukx_sync_b200 import build
     build.build()
