@@ -186,17 +186,20 @@ struct Shared {
 
 __device__ __forceinline__ uint32_t smem_of(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
 
+__device__ __forceinline__ bool phase_done(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok;
+}
 // Whether the phase `parity` of the barrier completed; gives up after some seconds, which only a
 // copy that never ends could bring about.
-__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity) {
-    for (int i = 0; i < (1 << 20); ++i) {
-        uint32_t ok;
-        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
-                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-        if (ok) return true;
-    }
+__device__ __noinline__ bool wait_longer(uint32_t bar, uint32_t parity) {
+    for (int i = 0; i < (1 << 20); ++i)
+        if (phase_done(bar, parity)) return true;
     return false;
 }
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity) { return phase_done(bar, parity) || wait_longer(bar, parity); }
 
 // The largest of a warp's values: as integers of the same order, one instruction for the warp.
 __device__ __forceinline__ float warp_max(float x) {
@@ -707,19 +710,17 @@ int fail(char* err, size_t errlen, int status, const std::string& msg) {
 
 // A row that does not fit the rings is read a second time for its gradient, out of L2 as long as the
 // rows that are being worked on at once are no more than this (of 126 MB; the gradients pass through
-// it too).  2143 MB of 4096 x 152k bf16 rows, a quarter masked: 0.39 ms with 45 MB of rows at once,
-// 0.48 with 90, 0.44 with 180; 2048 x 152k fp32 0.46, 0.57, 0.60.
+// it too).  4096 x 152k bf16 rows, 28% of them masked: 0.38 ms with 48 MB, 0.41 with 24 (more CTAs per
+// row wait for one another), 0.48 with 96; 2048 x 152k fp32: 0.45, 0.44, 0.55.
 constexpr int64_t kRowsAtOnce = int64_t(48) << 20;
 
-// A row by one warp, where nothing waits for another warp: rows that its ring holds, and longer ones
-// when there are enough of them to go round twice (16384 x 8192 bf16: 0.15 ms by CTAs of four warps).
-bool warp_rows(int64_t n, int64_t V, int vec) {
-    const int64_t bytes = V / vec * 16;
-    return bytes <= int64_t(kSlots) * kChunk * 16 ? n >= kRowGrid : n >= 2 * kMaxUnits && bytes * kMaxUnits <= kRowsAtOnce;
-}
+// A row by one warp, where nothing waits for another warp: rows short enough, and as many of them as
+// there are CTAs (2500 x 8192: 17 us against 21 by CTAs, 600 x 1024: 8 against 10); fewer rows are
+// shared out (200 x 8192: 9 us against 13 by warps).
+bool warp_rows(int64_t n, int64_t V, int vec) { return n >= kRowGrid && V / vec * 16 * kMaxUnits <= kRowsAtOnce; }
 
 // CTAs per row: enough to keep the rows at once in L2 (with a gradient), and as many as the rows leave
-// room for while a slice keeps two chunks per warp.
+// room for while a slice keeps a chunk per warp (64 x 152k: 15 us, with one CTA per row 37).
 int cluster_for(int64_t n, int64_t V, int vec, bool grad) {
     const int64_t bytes = V / vec * 16;
     int C = 1;
