@@ -16,6 +16,11 @@
 //                    is reduced; a row that fits its ring is turned into the gradient from there
 //   k_policy_sums    one CTA: the terms of the rows summed in a fixed order, in double
 //   k_policy_again   the gradient once more, scaled, from the rows' saved (u, R, s)
+//
+// Bounds: HBM where nothing interferes (without gradient 4096 x 152k rows, 894 MB that count, take
+// 0.142 ms, 6.3 TB/s; with it 2143 MB 0.38 ms, 5.6 TB/s).  What is left between that and the 6.5 of a
+// copy: rows that do not fit the rings come through L2 twice (without the second time 0.36 ms), and the
+// CTAs of a cluster wait for one another once a row.  Leaving the exponentials out changes nothing.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -36,6 +41,9 @@ namespace {
 
 namespace cg = cooperative_groups;
 
+// Sixteen warps per SM in CTAs of four, whose reductions pass under one another's streams: 4096 x 152k
+// rows with their gradient take 0.38 ms, by CTAs of two warps 0.39, of sixteen 0.40; with 24 or 32 warps
+// per SM and shorter rings 0.45 and 0.48.  Rings fill what shared memory there is.
 constexpr int kRowThreads = 128;
 constexpr int kRowWarps = kRowThreads / 32;
 constexpr int kMaxCluster = 8;
