@@ -622,44 +622,57 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) k_policy_rows(const __g
     }
 }
 
-// Every thread takes a run of rows; the counts before it give it its places among the rows that
-// count and among those that do not.
+// Every warp takes a run of rows, 32 * kAtOnce at a time; the counts before it give it its places among
+// the rows that count and among those that do not.
 __global__ void __launch_bounds__(1024) k_policy_plan(const __grid_constant__ crx_policy_args a) {
     __shared__ double red[32];
-    __shared__ int before[32];
-    const int n = int(a.batch * a.steps), steps = int(a.steps), tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-    const int per = (n + 1023) / 1024;
+    __shared__ uint32_t before[32];
+    constexpr uint32_t kAtOnce = 8;
+    const uint32_t n = uint32_t(a.batch * a.steps), steps = uint32_t(a.steps), lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const uint32_t per = (n / 32 + 32) / 32 * 32, lo = tmin(n, w * per), hi = tmin(n, lo + per);
     let_next_start();
-    const int lo = int(tmin<int64_t>(n, int64_t(tid) * per)), hi = int(tmin<int64_t>(n, int64_t(lo) + per));
+    const auto load = [&](uint32_t i, float* x) {   // weights i + lane, i + lane + 32, ...; 0 behind the run
+#pragma unroll
+        for (uint32_t k = 0; k < kAtOnce; ++k) {
+            const uint32_t row = i + 32 * k + lane;
+            x[k] = row < hi ? weight(a, row / steps, row % steps) : 0.f;
+        }
+    };
     double v = 0;
-    int c = 0;
-    for (int i = lo; i < hi; ++i) {
-        const float x = weight(a, i / steps, i % steps);
-        v += double(x);
-        c += x != 0.f;
+    uint32_t c = 0;
+    float x[kAtOnce];
+    for (uint32_t i = lo; i < hi; i += 32 * kAtOnce) {
+        load(i, x);
+#pragma unroll
+        for (uint32_t k = 0; k < kAtOnce; ++k) {
+            v += double(x[k]);
+            c += __popc(__ballot_sync(0xffffffffu, x[k] != 0.f));
+        }
     }
     v = warp_sum(v);
-    int incl = c;
-    for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
+    if (lane == 0) {
+        red[w] = v;
+        before[w] = c;
     }
-    if (lane == 31) before[w] = incl;
-    if (lane == 0) red[w] = v;
     __syncthreads();
-    const int mine = before[lane];
-    int total = mine, scan = mine;
+    const uint32_t mine = before[lane];
+    uint32_t scan = mine;
     for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, scan, o);
-        if (lane >= o) scan += y;
+        const uint32_t y = __shfl_up_sync(0xffffffffu, scan, o);
+        if (lane >= uint32_t(o)) scan += y;
     }
-    total = __shfl_sync(0xffffffffu, scan, 31);
-    int in = __shfl_sync(0xffffffffu, scan - mine, w) + incl - c;   // rows that count before this thread's
-    int out = total + lo - in;
+    const uint32_t total = __shfl_sync(0xffffffffu, scan, 31);
+    uint32_t in = __shfl_sync(0xffffffffu, scan - mine, w);   // rows that count before this warp's
     int32_t* order = order_of(a);
-    for (int i = lo; i < hi; ++i) {
-        if (weight(a, i / steps, i % steps) != 0.f) order[in++] = i;
-        else order[out++] = i;
+    for (uint32_t i = lo; i < hi; i += 32 * kAtOnce) {
+        load(i, x);
+#pragma unroll
+        for (uint32_t k = 0; k < kAtOnce; ++k) {
+            const uint32_t row = i + 32 * k + lane, yes = __ballot_sync(0xffffffffu, x[k] != 0.f);
+            const uint32_t at_in = in + __popc(yes & lanemask_lt());
+            if (row < hi) order[x[k] != 0.f ? at_in : total + row - at_in] = int32_t(row);   // (row - at_in do not count before it)
+            in += __popc(yes);
+        }
     }
     if (w == 0) {
         v = warp_sum(red[lane]);

@@ -469,6 +469,17 @@ def test_masks(crx, kind):
     verify(crx, batch(5, 9, 777, torch.bfloat16, 8, mask=mask), kl_coef=0.04, denom=5.0)
 
 
+@pytest.mark.parametrize("n", [1, 31, 32, 33, 255, 1023, 1024, 1025, 8191, 30001, 262147])
+def test_masks_over_many_rows(crx, n):
+    """The order in which rows are taken covers each once, wherever its runs end."""
+    mask = torch.rand(n, generator=gen(n)) < 0.5
+    d = batch(1, n, 5, torch.float32, 24, with_ref=False)
+    one = {k: v[0] if torch.is_tensor(v) else v for k, v in d.items()}
+    verify(crx, {**one, "mask": mask})
+    out, grad = run(crx, {**one, "mask": mask})
+    assert bool((grad.abs().sum(-1) != 0).cpu()[~mask].sum() == 0)
+
+
 def test_a_mask_that_leaves_nothing(crx):
     d = batch(2, 3, 100, torch.float32, 9, mask=torch.zeros(2, 3, dtype=torch.bool))
     out, grad = run(crx, d, kl_coef=0.04)
@@ -694,6 +705,26 @@ def test_elements_past_2_31(crx):
     near(out.logp[-4:], want["logp"][0], want["tol_logp"][0])
     near(g[-4:], want["grad"][0], want["tol_grad"][0])
     assert not g[:100].any() and not g[T // 2:T // 2 + 100].any() and not g[-104:-4].any()
+
+
+def test_gradients_past_2_31(crx):
+    n = (1 << 31) + 4099
+    g = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    g[-5000:] = 3.0
+    g[:7] = 4.0
+    want = math.sqrt(5000 * 9 + 7 * 16)
+    near(crx.grad_norm({"g": g}), want, want * ref.NORM)
+    p, m, v = (torch.zeros(n, device="cuda") for _ in range(3))
+    crx.adamw_step({"g": p}, {"g": g}, {"g": m}, {"g": v}, lr=1e-3, step=1)
+    for part in (slice(0, 5000), slice(n - 6000, n)):
+        x, z = g[part].cpu(), torch.zeros(p[part].numel())
+        new, tol = ref.adamw(z, x, z, z, lr=1e-3, step=1, b1=0.9, b2=0.999, eps=1e-8, wd=0.0)
+        for t, w, e in zip((p, m, v), new, tol):
+            near(t[part], w, e)
+    assert not p[n // 2:n // 2 + 100000].any()
+    crx.clip_grads({"g": g}, want / 2)
+    near(g[-5000:], *ref.clip(torch.full((5000,), 3.0, dtype=torch.bfloat16), ref.coef(want, want / 2)))
+    assert not g[n // 2:n // 2 + 100000].any()
 
 
 def test_calls_on_two_streams_and_equal_bits(crx):
