@@ -53,11 +53,14 @@ constexpr int kChunk = 128;            // 16-byte vectors of a slot: four per la
 constexpr int kRowGrid = 148 * kRowCtas;       // CTAs of the persistent grid
 constexpr int kMaxUnits = kRowGrid * kRowWarps;
 constexpr size_t kRingBytes = size_t(kRowWarps) * kSlots * kChunk * 16;
-constexpr float kFar = 3e38f;
+// Exponents are z c - R by one fma, exact but for its rounding, so at the maximum they are what R = M c lost
+// in its own rounding: at most 2^5 for |M c| below this bound, which a sum in fp32 bears (it cancels in p and in
+// logp) and beyond which 2^x soon overflows.  Larger maxima make a far row; what lies below -kFar adds nothing
+// to any other.
+constexpr float kFar = 0x1p30f;
 constexpr int kMaxDevices = 64;
 
-// 2^x to about 2 ulp; results below 2^-126 become 0, which neither a sum of at least 1 nor a
-// gradient in any of the types can tell from them.
+// 2^x to about 2 ulp; results below 2^-126 become 0: next to the maximum's term, 2^-32 or more, 2^-94 at most.
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -126,8 +129,9 @@ template <> __device__ __forceinline__ float vec_max<__half>(const uint4* q, int
     return fmaxf(__low2float(m), __high2float(m));
 }
 
-// The running (maximum, sum of 2^(z c - R)) of one thread, R = max(M c, -kFar).  The bound keeps R
-// finite where everything so far is -inf or the type's lowest value: those add 0.
+// The running (maximum, sum of 2^(z c - R)) of one thread, R = max(M c, -kFar).  The bound lets what
+// lies below it add 0 (-inf, the type's lowest value, any large negative number that rules tokens out),
+// also where nothing else has come yet.
 struct Running {
     float m = -INFINITY, r = -kFar, s = 0.f;
     __device__ __forceinline__ void raise(float top, float c) {
@@ -282,9 +286,9 @@ __device__ __forceinline__ float unit_total(float v, Shared& sh) {
     return v;
 }
 
-// The sum of a far row: one whose largest logit M is so large in magnitude that M c does not fit
-// fp32 (every logit the type's lowest value, say).  (z - M) c takes the place of z c - R, and each
-// CTA of the cluster goes over the whole row.
+// The sum of a far row: one whose largest logit M has |M c| >= kFar (every logit a large negative number, or
+// a temperature of 1e-8).  (z - M) c, which is 0 at the maximum, takes the place of z c - R, and each CTA of
+// the cluster goes over the whole row.
 template <class T, bool WARP>
 __device__ __noinline__ float far_sum(const T* z, int64_t V, float M, float c, Shared& sh) {
     float s = 0.f;

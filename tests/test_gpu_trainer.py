@@ -531,6 +531,82 @@ def test_rows_of_extreme_logits(crx, dtype, value):
     verify(crx, {**d, "logits": z}, temperature=0.5)
 
 
+# What a row's small probabilities may lose beside the tolerances of trainer_ref: 2^x is 0 below 2^-126, of
+# a sum that a maximum of up to 2^30 (in units of log2; its rounding is 2^5 at most) may have lowered to 2^-32.
+FLUSH = 2.0 ** -94
+
+
+def verify_rows(crx, d, tau=1.0):
+    """Loss, log-probabilities and gradient of rows without an older policy (so each ratio is 1, whatever
+    the log-probability), with the gradient's own error where a probability is as good as 0."""
+    out, grad = run(crx, d, temperature=tau)
+    want = ref.policy(d["logits"][..., :d["V"]], d["tokens"], d["adv"], tau=tau)
+    near(out.logp, want["logp"], want["tol_logp"], "logp")
+    near(out.loss, want["loss"], 4 * ref.H * float(d["adv"].abs().double().mean()) + 1e-12, "loss")
+    u = (d["adv"].double().expand(d["tokens"].shape) / d["tokens"].numel() / tau).abs()[..., None]
+    z = d["logits"][..., :d["V"]].double() / tau
+    p = torch.log_softmax(z, -1).exp()
+    hot = torch.zeros_like(p).scatter_(-1, d["tokens"][..., None], 1.0)
+    # u: advantage, 1 / number, 1 / temperature and their products; p: as in trainer_ref
+    depth = d["V"] / 512 + 48
+    expo = torch.where(p > 0, p.clamp(min=1e-300).log(), 0.0).abs() * 1.45
+    tol = u * (8 * ref.H * (hot + p) + p * ref.H * (depth + 20 + 4 * expo + 3 * math.log(d["V"])) + FLUSH) + ref.half_step(want["grad"], grad.dtype)
+    near(grad, want["grad"], tol, "grad")
+    return out, grad
+
+
+@pytest.mark.parametrize("fill", [1e7, 5e8, 1e9, 1e10, 1e12, 1e20, 1e30])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_vocabulary_masks_of_any_fill(crx, dtype, fill):
+    """Tokens ruled out by a large negative number: scattered ones, runs longer than a CTA's chunks, a row's first
+    and last elements; and rows of nothing but that number, or of the opposite one."""
+    V = 33333
+    d = batch(1, 8, V, dtype, 25, old=False, with_ref=False)
+    d["tokens"][:] = 20001
+    d["adv"] = torch.randn(1, 8, generator=gen(26))
+    z = d["logits"][0]
+    z[0, ::2] = -fill
+    z[1, :20000] = -fill
+    z[2, 20002:] = -fill
+    z[3, :9] = -fill
+    z[3, -9:] = -fill
+    z[4] = -fill
+    z[4, 20001] = 3.0
+    z[5] = -fill
+    z[6] = fill
+    z[7, 20001] = fill
+    verify_rows(crx, d)
+    warps = {**d, "logits": z[:7].repeat_interleave(100, 0)[None], "tokens": d["tokens"][:, :7].repeat_interleave(100, 1),
+             "adv": d["adv"][:, :7].repeat_interleave(100, 1)}
+    warps["logits"] = warps["logits"][..., 19000:20000 + 2048 + 3]   # as many short rows as take a warp each
+    verify_rows(crx, {**warps, "V": 3051, "tokens": warps["tokens"] - 19000})
+
+
+@pytest.mark.parametrize("tau", [1e-1, 1e-3, 1e-6, 1e-7, 1e-8, 1e-9, 1e-12, 1e-20, 2e-30, 1e4, 1e30])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_temperatures_down_to_the_limit(crx, dtype, tau):
+    """Ordinary logits; the largest was sampled, and in the last rows another."""
+    d = batch(1, 12, 1003, dtype, 27, old=False, with_ref=False)
+    d["tokens"] = d["logits"].argmax(-1)
+    d["tokens"][0, 8:] = 17
+    d["adv"] = torch.randn(1, 12, generator=gen(28))
+    verify_rows(crx, d, tau)
+
+
+@pytest.mark.parametrize("far", [1e-9, 1.0])
+def test_a_scaled_loss_of_large_logits(crx, far):
+    """The second pass over the logits takes the same exponents as the first."""
+    d = batch(1, 6, 1003, torch.float32, 43, old=False, with_ref=False)
+    if far == 1.0:
+        d["logits"][0, :3] *= 1e12
+        d["logits"][0, 4] = -1e10
+    z = d["logits"].cuda().requires_grad_()
+    out = crx.policy_loss(z, dev(d["tokens"]), dev(d["adv"]), temperature=far)
+    once, = torch.autograd.grad(out.loss, z, retain_graph=True)
+    twice, = torch.autograd.grad(out.loss * 2, z)
+    assert torch.isfinite(once).all() and torch.equal(twice, once * 2)
+
+
 def test_values_that_are_not_numbers(crx):
     d = batch(1, 4, 600, torch.float32, 13, old=False, with_ref=False)
     d["logits"][0, 1, 5] = math.nan
