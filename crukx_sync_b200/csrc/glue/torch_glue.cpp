@@ -239,6 +239,16 @@ bool rows(const at::Tensor& x, const at::Tensor& tokens, bool broadcast, crx_row
     *r = crx_rows{x.data_ptr(), s[0], s[1]};
     return true;
 }
+// Whether tensors that were saved came back as what they were.  Hooks may have moved them meanwhile
+// (offloading to the host), so addresses and strides are taken anew.
+bool same_again(const at::Tensor& logits, const at::Tensor& tokens, int dev, const crx_policy_args& a) {
+    const int64_t d = tokens.dim();
+    if ((d != 1 && d != 2) || logits.dim() != d + 1 || tokens.size(d - 1) != a.steps || (d == 2 ? tokens.size(0) : 1) != a.batch) return false;
+    if (!std::equal(tokens.sizes().begin(), tokens.sizes().end(), logits.sizes().begin()) || logits.size(d) != a.vocab) return false;
+    if (tokens.scalar_type() != (a.tokens64 ? at::kLong : at::kInt) || !type_bit(logits.scalar_type()) || type_code(logits.scalar_type()) != a.dtype) return false;
+    return logits.layout() == at::kStrided && (a.vocab == 1 || logits.stride(d) == 1) && logits.is_cuda() && logits.get_device() == dev &&
+           tokens.is_cuda() && tokens.get_device() == dev;
+}
 crx_rows wide_rows(const at::Tensor& x) {
     const int64_t d = x.dim();
     return crx_rows{x.data_ptr(), d == 3 ? x.stride(0) : 0, x.stride(d - 2)};
@@ -293,11 +303,13 @@ struct PolicyLossFn : public torch::autograd::Function<PolicyLossFn> {
         if (!scale.defined()) return {at::Tensor(), at::Tensor()};
         const auto saved = ctx->get_saved_variables();   // refuses tensors modified since
         const at::Tensor &logits = saved[0], &tokens = saved[1];
-        const int dev = logits.get_device();
-        const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
         crx_policy_args a;
         std::memcpy(&a, ctx->saved_data["args"].toStringRef().data(), sizeof a);
         const at::Tensor rows_kept = ctx->saved_data["rows"].toTensor();
+        const int dev = rows_kept.get_device();
+        TORCH_CHECK(same_again(logits, tokens, dev, a) && rows(tokens, tokens, false, &a.tokens),
+                    "policy_loss: saved logits or tokens came back with another shape, type or device");
+        const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
         c10::IValue& kept = ctx->saved_data["grad"];
         at::Tensor grad;
         const bool first = kept.isTensor();
@@ -309,7 +321,6 @@ struct PolicyLossFn : public torch::autograd::Function<PolicyLossFn> {
         }
         a.logits = wide_rows(logits);
         a.grad = wide_rows(grad);
-        a.tokens.p = tokens.data_ptr();
         a.rows = static_cast<float*>(rows_kept.data_ptr());
         a.logp = a.loss = a.stats = a.rows;   // results that this pass does not touch
         char err[512] = "";

@@ -1,6 +1,7 @@
 """policy_loss, grad_norm, clip_grads and adamw_step against their definitions in 64 bits, at the
 sizes, layouts, masks and values where they can go wrong, and run together as a trainer does."""
 
+import contextlib
 import math
 
 import pytest
@@ -740,6 +741,47 @@ def test_logits_changed_before_backward_are_noticed(crx):
         y.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         out.loss.backward()
+
+
+class Offloaded:
+    """Hooks that hand saved tensors to the backward pass as contiguous copies, as offloading them does."""
+
+    def __init__(self, there=lambda t: t.to("cpu", copy=True), back=lambda t: t.cuda()):
+        self.hooks = torch.autograd.graph.saved_tensors_hooks(lambda t: there(t.contiguous()), back)
+
+
+@pytest.mark.parametrize("scale", [1.0, 0.5])
+def test_saved_tensors_that_come_back_laid_out_otherwise(crx, scale):
+    """Shifted tokens and logits, saved by hooks that return contiguous ones."""
+    d = batch(4, 10, 301, torch.bfloat16, 29, mask=torch.rand(4, 10, generator=gen(30)) < 0.8)
+    z = d["logits"].cuda()
+    tokens, rest = dev(d["tokens"])[:, 1:], {k: dev(d[k])[:, 1:] for k in ("old", "ref", "mask")}
+
+    def grads(hooks):
+        x = z.clone().requires_grad_()
+        with hooks:
+            out = crx.policy_loss(x[:, :-1], tokens, dev(d["adv"]), old_logp=rest["old"], ref_logp=rest["ref"], mask=rest["mask"], kl_coef=0.04)
+        first, = torch.autograd.grad(out.loss * scale, x, retain_graph=True)
+        second, = torch.autograd.grad(out.loss * scale, x)
+        return first, second
+
+    want = grads(contextlib.nullcontext())
+    assert torch.equal(*want)
+    for hooks in (Offloaded().hooks, torch.autograd.graph.save_on_cpu(), torch.autograd.graph.save_on_cpu(pin_memory=True)):
+        for g, w in zip(grads(hooks), want):
+            assert torch.equal(g, w)
+
+
+@pytest.mark.parametrize("back", [lambda t: t, lambda t: t.cuda()[..., :1], lambda t: t.cuda().to(torch.int32 if t.dtype == torch.int64 else t.dtype),
+                                  lambda t: t.cuda().to(torch.float16 if t.dtype == torch.bfloat16 else t.dtype)],
+                         ids=["host", "shape", "tokens' type", "logits' type"])
+def test_saved_tensors_that_come_back_as_others_are_refused(crx, back):
+    d = batch(2, 5, 64, torch.bfloat16, 31)
+    z = d["logits"].cuda().requires_grad_()
+    with Offloaded(back=back).hooks:
+        out = crx.policy_loss(z, dev(d["tokens"]), dev(d["adv"]))
+    with pytest.raises(RuntimeError, match="saved"):
+        torch.autograd.grad(out.loss * 0.5, z)
 
 
 def test_gradient_against_differences(crx):
