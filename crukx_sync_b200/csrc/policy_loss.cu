@@ -579,7 +579,8 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) k_policy_rows(const __g
         const float A = r.advantage;
         const float ratio = a.old_logp.p ? expf(logp - r.old) : (logp == logp ? 1.f : logp);   // NaN logits show in the loss
         const bool clipped = (A > 0.f && ratio > 1.f + a.clip_high) || (A < 0.f && ratio < 1.f - a.clip_low);
-        const float gain = A == 0.f ? 0.f : (clipped ? (A > 0.f ? 1.f + a.clip_high : 1.f - a.clip_low) : ratio) * A;
+        // an advantage of 0 takes any ratio, infinite ones too, but what is not a number stays one
+        const float gain = A == 0.f && ratio == ratio ? 0.f : (clipped ? (A > 0.f ? 1.f + a.clip_high : 1.f - a.clip_low) : ratio) * A;
         float dl = clipped ? 0.f : -gain, k = 0.f;
         if (a.ref_logp.p) {
             const float x = r.ref - logp, e = expm1f(x);

@@ -627,6 +627,20 @@ def test_a_token_outside_the_vocabulary(crx, token):
     assert torch.isfinite(grad[0, ::2]).all()
 
 
+@pytest.mark.parametrize("what", ["token", "logits", "old"])
+def test_an_advantage_of_zero_hides_nothing(crx, what):
+    d = batch(1, 3, 600, torch.float32, 32, with_ref=False)
+    d["adv"] = torch.tensor([[1.0, 0.0, -1.0]])
+    if what == "token":
+        d["tokens"][0, 1] = 600
+    elif what == "logits":
+        d["logits"][0, 1, 7] = math.nan
+    else:
+        d["old"][0, 1] = math.nan
+    out, grad = run(crx, d)
+    assert torch.isnan(out.loss) and torch.isnan(grad[0, 1]).all() and torch.isfinite(grad[0, ::2]).all()
+
+
 def test_a_token_that_was_ruled_out(crx):
     """A sampled token of probability 0: logp -inf, ratio 0; without a KL term its gradient is finite."""
     d = batch(1, 2, 300, torch.float32, 15, with_ref=False)
