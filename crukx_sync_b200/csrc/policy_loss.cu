@@ -602,8 +602,12 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) k_policy_rows(const __g
             uint4* o = reinterpret_cast<uint4*>(g + sl.body) + first + lane;
             for (int k = 0, left = sl.hi - first; k < chunks; ++k, left -= in.kStride, o += in.kStride) {
                 uint4 q[4];
-                if (!fits) in.wait(in.at_);
+                const bool here = fits || in.wait(in.at_);
                 in.read(in.at_, q);
+                if (!here) {   // NaN in every type
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) q[v] = make_uint4(~0u, ~0u, ~0u, ~0u);
+                }
                 const int v0 = sl.hi - left + lane;
                 if (plain && left >= kChunk) {
 #pragma unroll
