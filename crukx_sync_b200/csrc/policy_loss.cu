@@ -198,20 +198,28 @@ struct Shared {
 
 __device__ __forceinline__ uint32_t smem_of(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
 
+// CLUSTER: what the phase counted was written by other CTAs of the cluster.
+template <bool CLUSTER>
 __device__ __forceinline__ bool phase_done(uint32_t bar, uint32_t parity) {
     uint32_t ok;
-    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
-                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if (CLUSTER)
+        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    else
+        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok;
 }
 // Whether the phase `parity` of the barrier completed; gives up after some seconds, which only a
 // copy that never ends could bring about.
+template <bool CLUSTER>
 __device__ __noinline__ bool wait_longer(uint32_t bar, uint32_t parity) {
     for (int i = 0; i < (1 << 20); ++i)
-        if (phase_done(bar, parity)) return true;
+        if (phase_done<CLUSTER>(bar, parity)) return true;
     return false;
 }
-__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity) { return phase_done(bar, parity) || wait_longer(bar, parity); }
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity) { return phase_done<CLUSTER>(bar, parity) || wait_longer<CLUSTER>(bar, parity); }
 
 // The largest of a warp's values: as integers of the same order, one instruction for the warp.
 __device__ __forceinline__ float warp_max(float x) {
@@ -267,7 +275,7 @@ __device__ __forceinline__ Running row_total(Running run, Shared& sh, uint32_t i
                          : "memory");
         }
     }
-    const bool here = wait_phase(came, (i >> 1) & 1);
+    const bool here = wait_phase<true>(came, (i >> 1) & 1);
     run = warp_total(lane_entry(sh.part[half], C), c);
     if (!here) run.s = NAN;
     return run;
