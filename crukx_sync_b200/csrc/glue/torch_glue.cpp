@@ -5,6 +5,7 @@
 // Arguments that do not fit make a function return None (or False) before anything is launched;
 // trainer.py then says which one it is.
 #include <c10/core/InferenceMode.h>
+#include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -282,9 +283,18 @@ Results run(Call& c, const at::Tensor& logits, bool want_grad) {
     return r;
 }
 
+// The graph that the device's current stream is being captured into, 0 for none.
+int64_t capture_of(int dev) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    C10_CUDA_CHECK(cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream_of(dev)), &status, &id));
+    return status == cudaStreamCaptureStatusActive ? static_cast<int64_t>(id) : 0;
+}
+
 // The forward pass leaves the gradient for an incoming gradient of 1.  The backward pass hands it
 // out; for another one (and the second time) it is computed again from the logits, so that it is
-// rounded once whatever its scale.
+// rounded once whatever its scale.  Also where only one of the passes runs again: a replayed backward
+// pass finds what it left the time before, and a replayed loss would write into what was handed out.
 struct PolicyLossFn : public torch::autograd::Function<PolicyLossFn> {
     static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits, Call* c) {
         Results r = run(*c, logits, true);
@@ -293,6 +303,7 @@ struct PolicyLossFn : public torch::autograd::Function<PolicyLossFn> {
         ctx->saved_data["args"] = std::string(reinterpret_cast<const char*>(&c->a), sizeof c->a);
         ctx->saved_data["rows"] = r.rows;
         ctx->saved_data["grad"] = r.grad;
+        ctx->saved_data["capture"] = capture_of(c->dev);
         ctx->mark_non_differentiable({r.logp, stats[0], stats[1]});
         ctx->set_materialize_grads(false);
         return {r.loss, r.logp, stats[0], stats[1]};
@@ -312,7 +323,7 @@ struct PolicyLossFn : public torch::autograd::Function<PolicyLossFn> {
         const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
         c10::IValue& kept = ctx->saved_data["grad"];
         at::Tensor grad;
-        const bool first = kept.isTensor();
+        const bool first = kept.isTensor() && ctx->saved_data["capture"].toInt() == capture_of(dev);
         if (first) {
             grad = kept.toTensor();
             kept = c10::IValue();

@@ -920,6 +920,62 @@ def test_two_captured_losses(crx):
             near(g, want["grad"], want["tol_grad"])
 
 
+def test_a_backward_pass_captured_without_its_loss(crx):
+    """Each replay gives the gradient for the incoming gradient of that time, whatever was done with the one before."""
+    d = batch(2, 12, 900, torch.bfloat16, 33)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for captured in (False, True):
+        with torch.cuda.stream(side):
+            z = d["logits"].cuda().requires_grad_()
+            args = [dev(d["tokens"]), dev(d["adv"])]
+            old, scale = dev(d["old"]), torch.ones((), device="cuda")
+            want = {}
+            for f in (1.0, 2.0, -0.5):
+                out = crx.policy_loss(z, *args, old_logp=old)
+                want[f], = torch.autograd.grad(out.loss, z, grad_outputs=torch.tensor(f, device="cuda"))
+            first = torch.cuda.CUDAGraph()
+            if captured:
+                with torch.cuda.graph(first, stream=side):
+                    out = crx.policy_loss(z, *args, old_logp=old)
+                first.replay()
+            else:
+                out = crx.policy_loss(z, *args, old_logp=old)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                g, = torch.autograd.grad(out.loss, z, grad_outputs=scale, retain_graph=True)
+            for f in (2.0, 1.0, 1.0, -0.5, 1.0):
+                scale.fill_(f)
+                graph.replay()
+                assert torch.equal(g, want[f]), (captured, f)
+                g.zero_()   # the caller's own
+            if captured:   # a gradient taken outside stays as it is when the loss is replayed on other logits
+                kept, = torch.autograd.grad(out.loss, z, retain_graph=True)
+                assert torch.equal(kept, want[1.0])
+                with torch.no_grad():
+                    z.zero_()
+                first.replay()
+                assert torch.equal(kept, want[1.0])
+        torch.cuda.synchronize()
+
+
+def test_a_graphed_callable(crx):
+    """Loss and backward pass captured one after the other, replayed on new inputs."""
+    shape = (2, 9, 701)
+    d = batch(*shape, torch.bfloat16, 34, with_ref=False)
+    tokens, adv, old = dev(d["tokens"]), dev(d["adv"]), dev(d["old"])
+    z = d["logits"].cuda().requires_grad_()
+    graphed = torch.cuda.make_graphed_callables(lambda x: crx.policy_loss(x, tokens, adv, old_logp=old).loss, (z,))
+    for seed, f in ((35, 1.0), (36, 3.0), (37, 1.0)):
+        x = batch(*shape, torch.bfloat16, seed)["logits"].cuda().requires_grad_()
+        loss = graphed(x)
+        g, = torch.autograd.grad(loss * f, x)
+        y = x.detach().clone().requires_grad_()
+        out = crx.policy_loss(y, tokens, adv, old_logp=old)
+        w, = torch.autograd.grad(out.loss * f, y)
+        assert torch.equal(loss, out.loss) and torch.equal(g, w)
+
+
 # ---------------------------------------------------------------------------------- together
 
 def test_a_trainers_step_through_to_the_worker(crx):
