@@ -522,7 +522,8 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) k_policy_rows(const __g
     else __syncthreads();
     after_previous();
     const float c = float(1.4426950408889634 / double(a.temperature));
-    const float inv_d = float(inv_denom < 0 ? plan_of(a)->inv_denom : inv_denom), inv_tau = 1.f / a.temperature;
+    const double inv_d = inv_denom < 0 ? plan_of(a)->inv_denom : inv_denom;   // weights may sum to what fp32 has no reciprocal of
+    const float inv_tau = 1.f / a.temperature;
     const int32_t* order = planned ? order_of(a) : nullptr;
     const uint32_t counted = planned ? uint32_t(plan_of(a)->counted) : n;
     double loss = 0, kl = 0, cut = 0;
@@ -595,12 +596,12 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) k_policy_rows(const __g
             k = e - x;
             if (a.kl_coef != 0.f) dl -= a.kl_coef * e;   // (a k that is only reported may overflow)
         }
-        const float u = w * inv_d * dl * inv_tau;
+        const float u = float(double(w) * inv_d) * dl * inv_tau;
         if (rank == 0 && tid == 0) {
             a.logp[row] = logp;
             saved_of(a)[row] = make_float4(u, R, s, far ? 1.f : 0.f);
-            loss += double(w * ((a.kl_coef != 0.f ? a.kl_coef * k : 0.f) - gain));
-            kl += double(w * k);
+            loss += double(w) * double((a.kl_coef != 0.f ? a.kl_coef * k : 0.f) - gain);
+            kl += double(w) * double(k);
             cut += double(clipped ? w : 0.f);
         }
         if (GRAD) {

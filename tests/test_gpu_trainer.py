@@ -470,6 +470,16 @@ def test_masks(crx, kind):
     verify(crx, batch(5, 9, 777, torch.bfloat16, 8, mask=mask), kl_coef=0.04, denom=5.0)
 
 
+@pytest.mark.parametrize("size", [1e-41, 1e-30, 1e30, 1e38])
+def test_weights_of_any_size(crx, size):
+    """Weights and their sum far from 1: only their proportions count."""
+    d = batch(2, 8, 500, torch.float32, 38)
+    steps = torch.randint(1, 4, (2, 8), generator=gen(39)).float()
+    mask = steps * torch.tensor(size)
+    verify(crx, {**d, "mask": mask}, kl_coef=0.04)
+    verify(crx, {**d, "mask": mask}, kl_coef=0.04, denom=float(mask.double().sum()) / 2)
+
+
 @pytest.mark.parametrize("n", [1, 31, 32, 33, 255, 1023, 1024, 1025, 8191, 30001, 262147])
 def test_masks_over_many_rows(crx, n):
     """The order in which rows are taken covers each once, wherever its runs end."""
