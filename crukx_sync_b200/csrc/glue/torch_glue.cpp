@@ -4,6 +4,7 @@
 //
 // Arguments that do not fit make a function return None (or False) before anything is launched;
 // trainer.py then says which one it is.
+#include <c10/core/AutogradState.h>
 #include <c10/core/InferenceMode.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -353,6 +354,7 @@ py::object policy_loss(const at::Tensor& logits, const at::Tensor& tokens, const
     if (!tokens.is_cuda() || tokens.get_device() != logits.get_device() || advantages.scalar_type() != at::kFloat ||
         (tokens.scalar_type() != at::kLong && tokens.scalar_type() != at::kInt))
         return py::none();
+    if (logits._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode()) return py::none();
     Call c = {};
     crx_policy_args& a = c.a;
     c.tokens = tokens;

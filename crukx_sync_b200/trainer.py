@@ -208,7 +208,8 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, advantages: torch.Te
     A token outside the vocabulary that counts makes the loss NaN.
 
     Where the logits require a gradient it is computed in this same call (they are read once), for
-    loss.backward() as it stands; a loss that is scaled first is right too, and costs a second pass."""
+    loss.backward() as it stands; a loss that is scaled first is right too, and costs a second pass.
+    Forward-mode gradients are refused."""
     lo, hi = clip
     if not (lo >= 0 and hi >= 0):
         raise ValueError(f"clip bounds must not be negative, got {clip}")
@@ -243,6 +244,8 @@ def _check_policy(logits, tokens, **given) -> None:
         raise ValueError("logits: the vocabulary must be contiguous")
     if not logits.is_cuda:
         raise ValueError("logits: expected a CUDA tensor")
+    if torch.autograd.forward_ad.unpack_dual(logits).tangent is not None:
+        raise ValueError("logits: forward-mode gradients are not supported")
     for what, t in (("tokens", tokens), *given.items()):
         if t is None:
             continue

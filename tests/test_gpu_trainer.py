@@ -743,6 +743,20 @@ def test_a_gradient_of_the_gradient_is_refused(crx):
         torch.autograd.grad(out.loss, z, create_graph=True)
 
 
+@pytest.mark.parametrize("needs_grad", [False, True])
+def test_forward_gradients_are_refused(crx, needs_grad):
+    from torch.autograd import forward_ad
+    d = batch(1, 2, 50, torch.float32, 40)
+    z = d["logits"].cuda().requires_grad_(needs_grad)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(z, torch.ones_like(z))
+        with pytest.raises(ValueError, match="forward"):
+            crx.policy_loss(dual, dev(d["tokens"]), dev(d["adv"]))
+        with pytest.raises(ValueError, match="forward"), torch.no_grad():
+            crx.policy_loss(dual, dev(d["tokens"]), dev(d["adv"]))
+    crx.policy_loss(z, dev(d["tokens"]), dev(d["adv"]))
+
+
 def test_inference_tensors_are_not_written(crx):
     with torch.inference_mode():
         t = torch.ones(8, device="cuda")

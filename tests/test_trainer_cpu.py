@@ -95,6 +95,16 @@ def test_loss_arguments_that_are_refused():
             call(**kw)
 
 
+@pytest.mark.parametrize("quiet", [False, True])
+def test_forward_gradients_are_refused(quiet):
+    """Without gradients of the backward kind too: no_grad does not stop the forward kind."""
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level():
+        z = forward_ad.make_dual(fake(2, 3, 8), torch.ones(2, 3, 8))
+        with pytest.raises(ValueError, match="forward"), torch.set_grad_enabled(not quiet):
+            crx.policy_loss(z, fake(2, 3, dtype=torch.int64), fake(2, 1))
+
+
 def test_gradient_memory_follows_the_logits(lib):
     glue = _ext.glue()
     base = torch.zeros(3, 5, 20, dtype=torch.bfloat16)
