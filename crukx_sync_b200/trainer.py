@@ -27,6 +27,7 @@ import torch
 from . import _ext
 from .codec import _cuda_device
 
+_LEAST = 2.0 ** -149   # of fp32: a positive number below it would be 0 there
 _GRADS, _F32, _BF16 = (torch.bfloat16, torch.float16, torch.float32), (torch.float32,), (torch.bfloat16,)
 
 
@@ -115,8 +116,8 @@ def clip_grads(grads: Mapping[str, torch.Tensor], max_norm: float, *, out: Mappi
     device) takes the place of the gradients' own, for gradients spread over ranks
     (dist.grad_norm_global).  A norm that is not finite is not clipped away: it leaves NaN, as its
     product says.  Tensors that share memory (a tied weight under two names) are refused."""
-    if not max_norm > 0:   # (NaN too)
-        raise ValueError(f"max_norm must be positive, got {max_norm}")
+    if not max_norm >= _LEAST:   # (NaN too)
+        raise ValueError(f"max_norm must be positive (in fp32), got {max_norm}")
     grads = _dict("gradients", grads)
     if out is not None:
         out = _dict("out", out)
@@ -153,8 +154,8 @@ def adamw_step(masters: Mapping[str, torch.Tensor], grads: Mapping[str, torch.Te
         raise ValueError(f"eps must be positive, got {eps}")
     if not math.isfinite(weight_decay):
         raise ValueError(f"weight_decay must be finite, got {weight_decay}")
-    if max_norm is not None and (norm is None or not max_norm > 0):
-        raise ValueError("max_norm must be positive and comes with norm")
+    if max_norm is not None and (norm is None or not max_norm >= _LEAST):
+        raise ValueError(f"max_norm must be positive (in fp32) and comes with norm, got {max_norm}")
     lr, lr_t = (0.0, lr) if isinstance(lr, torch.Tensor) else (lr, None)
     step, step_t = (1, step) if isinstance(step, torch.Tensor) else (step, None)
     if step < 1:

@@ -95,6 +95,16 @@ def test_loss_arguments_that_are_refused():
             call(**kw)
 
 
+@pytest.mark.parametrize("max_norm", [1e-46, 1e-300])
+def test_limits_that_fp32_does_not_hold(max_norm):
+    """Not taken as 0, which would mean that nothing is clipped."""
+    d = {"a": fake(4)}
+    with pytest.raises(ValueError, match="max_norm"):
+        crx.clip_grads(d, max_norm)
+    with pytest.raises(ValueError, match="max_norm"):
+        crx.adamw_step(d, {"a": fake(4)}, d, d, lr=1e-3, step=1, norm=fake(()), max_norm=max_norm)
+
+
 @pytest.mark.parametrize("quiet", [False, True])
 def test_forward_gradients_are_refused(quiet):
     """Without gradients of the backward kind too: no_grad does not stop the forward kind."""
