@@ -610,7 +610,10 @@ int crx_adamw_step(int32_t n, float* const* master, const void* const* grads, co
         if (const int s = check_common("crx_adamw_step", n, grads, dtypes, numel, err, errlen)) return s;
         if (!args || (n && (!master || !exp_avg || !exp_avg_sq))) return fail(err, errlen, CRX_BAD_ARGUMENT, "crx_adamw_step: null pointer");
         if (!(args->beta1 >= 0 && args->beta1 < 1 && args->beta2 >= 0 && args->beta2 < 1)) return fail(err, errlen, CRX_VALUE_ERROR, "betas must be in [0, 1)");
-        if (!(args->eps > 0)) return fail(err, errlen, CRX_VALUE_ERROR, "eps must be positive");
+        // in fp32, as the kernel takes them
+        if (!(float(args->eps) > 0)) return fail(err, errlen, CRX_VALUE_ERROR, "eps must be positive");
+        if (!std::isfinite(float(args->weight_decay)) || (!args->lr_p && !std::isfinite(float(args->lr))))
+            return fail(err, errlen, CRX_VALUE_ERROR, "lr and weight_decay must be finite");
         if (!args->step_p && args->step < 1) return fail(err, errlen, CRX_VALUE_ERROR, "step counts from 1");
         std::vector<Range> r;
         r.reserve(size_t(n) * 5);

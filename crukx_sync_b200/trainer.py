@@ -27,7 +27,7 @@ import torch
 from . import _ext
 from .codec import _cuda_device
 
-_LEAST = 2.0 ** -149   # of fp32: a positive number below it would be 0 there
+_LEAST, _MOST = 2.0 ** -149, torch.finfo(torch.float32).max   # of fp32: beyond them a number would be 0 or infinite there
 _GRADS, _F32, _BF16 = (torch.bfloat16, torch.float16, torch.float32), (torch.float32,), (torch.bfloat16,)
 
 
@@ -150,18 +150,18 @@ def adamw_step(masters: Mapping[str, torch.Tensor], grads: Mapping[str, torch.Te
     b1, b2 = betas
     if not (0 <= b1 < 1 and 0 <= b2 < 1):
         raise ValueError(f"betas must be in [0, 1), got {betas}")
-    if not eps > 0:
-        raise ValueError(f"eps must be positive, got {eps}")
-    if not math.isfinite(weight_decay):
-        raise ValueError(f"weight_decay must be finite, got {weight_decay}")
+    if not eps >= _LEAST:
+        raise ValueError(f"eps must be positive (in fp32), got {eps}")
+    if not abs(weight_decay) <= _MOST:
+        raise ValueError(f"weight_decay must be finite (in fp32), got {weight_decay}")
     if max_norm is not None and (norm is None or not max_norm >= _LEAST):
         raise ValueError(f"max_norm must be positive (in fp32) and comes with norm, got {max_norm}")
     lr, lr_t = (0.0, lr) if isinstance(lr, torch.Tensor) else (lr, None)
     step, step_t = (1, step) if isinstance(step, torch.Tensor) else (step, None)
     if step < 1:
         raise ValueError(f"step counts from 1, got {step}")
-    if not math.isfinite(lr):
-        raise ValueError(f"lr must be finite, got {lr}")
+    if not abs(lr) <= _MOST:
+        raise ValueError(f"lr must be finite (in fp32), got {lr}")
     grads, masters = _dict("gradients", grads), _dict("masters", masters)
     exp_avg, exp_avg_sq = _dict("exp_avg", exp_avg), _dict("exp_avg_sq", exp_avg_sq)
     if weights is not None:

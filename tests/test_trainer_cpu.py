@@ -179,6 +179,18 @@ def test_c_entry_points_refuse(lib):
     assert lib.crx_policy_loss(None, None, err, 512) == 5 and lib.crx_policy_backward(None, None, 0, None, err, 512) == 5
 
 
+@pytest.mark.parametrize("kw", [dict(eps=1e-46), dict(lr=1e39), dict(lr=-1e39), dict(weight_decay=1e39)], ids=str)
+def test_step_numbers_that_fp32_does_not_hold(lib, kw):
+    """An eps that would be 0 and rates that would be infinite, in Python and at the C entry."""
+    d = {"a": fake(4)}
+    with pytest.raises(ValueError, match=next(iter(kw))):
+        crx.adamw_step(d, {"a": fake(4)}, d, d, **{"lr": 1e-3, "step": 1, **kw})
+    err = ctypes.create_string_buffer(512)
+    args = struct.pack("5d4qf4x", kw.get("lr", 1e-3), 0.9, 0.99, kw.get("eps", 1e-8), kw.get("weight_decay", 0.0), 1, 0, 0, 0, 0.0)
+    assert lib.crx_adamw_step(1, pointers(4096), pointers(8192), _ext.CBuf("i", [2]), pointers(12288), pointers(16384), pointers(20480),
+                              _ext.CBuf("q", [4]), args, None, err, 512) == _ext.CRX_VALUE_ERROR and err.value
+
+
 def _rank(rank, world, port, queue):
     import os
 
