@@ -19,6 +19,7 @@ runs.  Caller mistakes are ValueErrors, raised before anything is launched.
 from __future__ import annotations
 
 import math
+import operator
 from collections.abc import Mapping
 from dataclasses import dataclass
 
@@ -41,6 +42,35 @@ def _dict(what: str, d) -> dict:
     if not isinstance(d, Mapping):
         raise ValueError(f"{what} must be a dict of name -> tensor, got {type(d)}")
     return dict(d)
+
+
+def _real(what: str, x) -> float:
+    if type(x) is float:
+        return x
+    try:
+        if not isinstance(x, (str, bytes, bytearray)):
+            return float(x)
+    except (TypeError, ValueError, OverflowError, RuntimeError):
+        pass
+    raise ValueError(f"{what}: expected a number, got {type(x)}")
+
+
+def _reals(what: str, x) -> tuple[float, float]:
+    try:
+        a, b = x
+    except (TypeError, ValueError):
+        raise ValueError(f"{what}: expected two numbers, got {x!r}") from None
+    return _real(what, a), _real(what, b)
+
+
+def _count(what: str, x) -> int:
+    try:
+        n = x if type(x) is int else operator.index(x)
+    except TypeError:
+        raise ValueError(f"{what}: expected an int, got {type(x)}") from None
+    if not 1 <= n < 1 << 63:
+        raise ValueError(f"{what} counts from 1, got {n}")
+    return n
 
 
 def _empty_device(grads) -> int:
@@ -116,6 +146,7 @@ def clip_grads(grads: Mapping[str, torch.Tensor], max_norm: float, *, out: Mappi
     device) takes the place of the gradients' own, for gradients spread over ranks
     (dist.grad_norm_global).  A norm that is not finite is not clipped away: it leaves NaN, as its
     product says.  Tensors that share memory (a tied weight under two names) are refused."""
+    max_norm = _real("max_norm", max_norm)
     if not max_norm >= _LEAST:   # (NaN too)
         raise ValueError(f"max_norm must be positive (in fp32), got {max_norm}")
     grads = _dict("gradients", grads)
@@ -147,19 +178,20 @@ def adamw_step(masters: Mapping[str, torch.Tensor], grads: Mapping[str, torch.Te
     is not finite, masters and moments stay as they are (weights get the masters' rounding all the
     same).  `lr` (fp32) and `step` (int64) may be one-element tensors on the device, read when the
     step runs: a captured graph then follows them.  Memory that the step writes may not be shared."""
-    b1, b2 = betas
+    b1, b2 = _reals("betas", betas)
+    eps, weight_decay = _real("eps", eps), _real("weight_decay", weight_decay)
     if not (0 <= b1 < 1 and 0 <= b2 < 1):
         raise ValueError(f"betas must be in [0, 1), got {betas}")
     if not eps >= _LEAST:
         raise ValueError(f"eps must be positive (in fp32), got {eps}")
     if not abs(weight_decay) <= _MOST:
         raise ValueError(f"weight_decay must be finite (in fp32), got {weight_decay}")
-    if max_norm is not None and (norm is None or not max_norm >= _LEAST):
-        raise ValueError(f"max_norm must be positive (in fp32) and comes with norm, got {max_norm}")
-    lr, lr_t = (0.0, lr) if isinstance(lr, torch.Tensor) else (lr, None)
-    step, step_t = (1, step) if isinstance(step, torch.Tensor) else (step, None)
-    if step < 1:
-        raise ValueError(f"step counts from 1, got {step}")
+    if max_norm is not None:
+        max_norm = _real("max_norm", max_norm)
+        if norm is None or not max_norm >= _LEAST:
+            raise ValueError(f"max_norm must be positive (in fp32) and comes with norm, got {max_norm}")
+    lr, lr_t = (0.0, lr) if isinstance(lr, torch.Tensor) else (_real("lr", lr), None)
+    step, step_t = (1, step) if isinstance(step, torch.Tensor) else (_count("step", step), None)
     if not abs(lr) <= _MOST:
         raise ValueError(f"lr must be finite (in fp32), got {lr}")
     grads, masters = _dict("gradients", grads), _dict("masters", masters)
@@ -211,7 +243,8 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, advantages: torch.Te
     Where the logits require a gradient it is computed in this same call (they are read once), for
     loss.backward() as it stands; a loss that is scaled first is right too, and costs a second pass.
     Forward-mode gradients are refused."""
-    lo, hi = clip
+    lo, hi = _reals("clip", clip)
+    temperature, kl_coef = _real("temperature", temperature), _real("kl_coef", kl_coef)
     if not (lo >= 0 and hi >= 0):
         raise ValueError(f"clip bounds must not be negative, got {clip}")
     if not 1e-30 < temperature < math.inf:   # (1 / temperature is a number fp32 holds)
@@ -220,8 +253,10 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, advantages: torch.Te
         raise ValueError(f"kl_coef must be less than 1e30, got {kl_coef}")
     if kl_coef and ref_logp is None:
         raise ValueError("kl_coef needs ref_logp")
-    if denom is not None and not denom > 0:
-        raise ValueError(f"denom must be positive, got {denom}")
+    if denom is not None:
+        denom = _real("denom", denom)
+        if not denom > 0:
+            raise ValueError(f"denom must be positive, got {denom}")
     given = dict(tokens=tokens, advantages=advantages, old_logp=old_logp, ref_logp=ref_logp, mask=mask)
     for what, t in (("logits", logits), *given.items()):
         if t is None and what in ("logits", "tokens", "advantages"):

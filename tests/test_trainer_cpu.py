@@ -105,6 +105,47 @@ def test_limits_that_fp32_does_not_hold(max_norm):
         crx.adamw_step(d, {"a": fake(4)}, d, d, lr=1e-3, step=1, norm=fake(()), max_norm=max_norm)
 
 
+def test_values_that_are_no_numbers_are_value_errors():
+    d, z = {"a": fake(4)}, fake(2, 3, 8)
+    words = ["1e-3", None, object(), 1j, [1.0], 10 ** 400]
+    for bad in words:
+        with pytest.raises(ValueError, match="max_norm"):
+            crx.clip_grads(d, bad)
+        for name in ("lr", "step", "eps", "weight_decay", "betas", "max_norm"):
+            if (name, bad) == ("max_norm", None):
+                continue   # (no clipping)
+            kw = {"lr": 1e-3, "step": 1, "norm": fake(()), name: (0.9, bad) if name == "betas" else bad}
+            with pytest.raises(ValueError, match=name):
+                crx.adamw_step(d, {"a": fake(4)}, d, d, **kw)
+        for name in ("clip", "kl_coef", "temperature", "denom"):
+            if (name, bad) == ("denom", None):
+                continue   # (the sum of the mask)
+            kw = {"ref_logp": fake(2, 3), name: (bad, 0.2) if name == "clip" else bad}
+            with pytest.raises(ValueError, match=name):
+                crx.policy_loss(z, fake(2, 3, dtype=torch.int64), fake(2, 1), **kw)
+    for bad in (2.5, 1 << 63, -(1 << 63)):
+        with pytest.raises(ValueError, match="step"):
+            crx.adamw_step(d, {"a": fake(4)}, d, d, lr=1e-3, step=bad)
+    for bad in (0.9, None, (0.9,), (0.9, 0.99, 0.999)):
+        with pytest.raises(ValueError, match="betas"):
+            crx.adamw_step(d, {"a": fake(4)}, d, d, lr=1e-3, step=1, betas=bad)
+        with pytest.raises(ValueError, match="clip"):
+            crx.policy_loss(z, fake(2, 3, dtype=torch.int64), fake(2, 1), clip=bad)
+
+
+def test_numbers_of_other_types_are_taken():
+    """Integers, numpy's and torch's numbers get as far as the tensors."""
+    import numpy as np
+    d = {"a": fake(4)}
+    for one, half in ((np.int64(1), np.float32(0.5)), (True, np.float64(0.5)), (1, torch.tensor(0.5))):
+        with pytest.raises(ValueError, match="these tensors"):
+            crx.adamw_step(d, {"a": fake(4)}, d, d, lr=half if not isinstance(half, torch.Tensor) else 1, step=one, betas=(half, half), eps=half,
+                           weight_decay=half, norm=fake(()), max_norm=half)
+        with pytest.raises(ValueError, match="these tensors"):
+            crx.policy_loss(fake(2, 3, 8), fake(2, 3, dtype=torch.int64), fake(2, 1), ref_logp=fake(2, 3), clip=(half, one), kl_coef=half,
+                            temperature=half, denom=one)
+
+
 @pytest.mark.parametrize("quiet", [False, True])
 def test_forward_gradients_are_refused(quiet):
     """Without gradients of the backward kind too: no_grad does not stop the forward kind."""
