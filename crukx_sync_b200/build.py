@@ -4,13 +4,16 @@ torch side of trainer.py's calls, ``crukx_sync_b200/_glue.so``, with g++.
     python -m crukx_sync_b200.build [--force] [--verbose]
 
 Objects go to ``crukx_sync_b200/_build/``; a file is recompiled when it or any header is newer
-than its object.  The library exports the C ABI declared in ``include/crukx_b200.h``.
+than its object.  The library exports the C ABI declared in ``include/crukx_b200.h``.  The torch side is
+compiled again for another torch or Python too; where it cannot be (no headers of theirs), that is
+reported and the library stands: the codec does without it, and trainer.py's calls say what is missing.
 """
 
 from __future__ import annotations
 
 import concurrent.futures
 import glob
+import importlib.metadata
 import importlib.util
 import os
 import shutil
@@ -25,6 +28,7 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libcrukx_b200.so")
 GLUE_SRC = os.path.join(CSRC, "glue", "torch_glue.cpp")
 GLUE = os.path.join(HERE, "_glue.so")
+GLUE_BUILT = os.path.join(BUILD, "glue.built")   # what it was built for
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O3", "-I", os.path.join(ROOT, "include"),
          "--expt-relaxed-constexpr"]
@@ -47,7 +51,10 @@ def _headers():
 
 
 def glue_command(out: str) -> list[str]:
-    torch = os.path.dirname(importlib.util.find_spec("torch").origin)   # (found, not imported: that takes a while)
+    spec = importlib.util.find_spec("torch")   # (found, not imported: that takes a while)
+    if spec is None:
+        raise RuntimeError("torch not found")
+    torch = os.path.dirname(spec.origin)
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
     include = [os.path.join(torch, "include"), os.path.join(torch, "include", "torch", "csrc", "api", "include"),
                sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
@@ -55,6 +62,22 @@ def glue_command(out: str) -> list[str]:
             *[x for d in include for x in ("-I", d)], GLUE_SRC, "-o", out, "-L", HERE, "-l:libcrukx_b200.so",
             "-L", os.path.join(torch, "lib"), "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
             "-Wl,-rpath,$ORIGIN"]
+
+
+def build_glue(run, force: bool = False) -> None:
+    built_for = f"torch {importlib.metadata.version('torch')}, {sysconfig.get_config_var('SOABI')}\n"
+    newest = max(os.path.getmtime(GLUE_SRC), os.path.getmtime(os.path.join(ROOT, "include", "crukx_b200.h")))
+    if not force and os.path.exists(GLUE) and os.path.getmtime(GLUE) >= newest and os.path.exists(GLUE_BUILT):
+        with open(GLUE_BUILT) as f:
+            if f.read() == built_for:
+                return
+    if os.path.exists(GLUE):
+        os.remove(GLUE)   # not left behind when the compiler fails
+    tmp = GLUE + ".tmp"
+    run(glue_command(tmp))
+    os.replace(tmp, GLUE)
+    with open(GLUE_BUILT, "w") as f:
+        f.write(built_for)
 
 
 def build(force: bool = False, verbose: bool = False, extra: list[str] | None = None) -> str:
@@ -90,11 +113,10 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
         tmp = LIB + ".tmp"
         run([cc, *ARCH, "-shared", "-o", tmp, *objs, "-lcudart"])
         os.replace(tmp, LIB)
-    header = os.path.join(ROOT, "include", "crukx_b200.h")
-    if force or not os.path.exists(GLUE) or os.path.getmtime(GLUE) < max(os.path.getmtime(GLUE_SRC), os.path.getmtime(header)):
-        tmp = GLUE + ".tmp"
-        run(glue_command(tmp))
-        os.replace(tmp, GLUE)
+    try:
+        build_glue(run, force)
+    except (RuntimeError, OSError, importlib.metadata.PackageNotFoundError) as exc:
+        print(f"crukx_sync_b200: _glue.so was not built, trainer.py's calls will not run: {exc}", file=sys.stderr, flush=True)
     return LIB
 
 

@@ -232,6 +232,44 @@ def test_step_numbers_that_fp32_does_not_hold(lib, kw):
                               _ext.CBuf("q", [4]), args, None, err, 512) == _ext.CRX_VALUE_ERROR and err.value
 
 
+@pytest.fixture
+def glue_files(tmp_path, monkeypatch):
+    """A build whose torch side is one made-up source and whose compiler copies it."""
+    from crukx_sync_b200 import build
+    build.build()
+    for name in ("GLUE", "GLUE_SRC", "GLUE_BUILT"):
+        monkeypatch.setattr(build, name, str(tmp_path / name))
+    (tmp_path / "GLUE_SRC").write_text("one")
+    monkeypatch.setattr(build, "glue_command", lambda out: ["cp", build.GLUE_SRC, out])
+    return build, tmp_path
+
+
+def test_the_torch_side_is_built_again_for_another_torch(glue_files, monkeypatch):
+    build, tmp = glue_files
+    build.build()
+    assert (tmp / "GLUE").read_text() == "one"
+    (tmp / "GLUE").write_text("kept")
+    build.build()
+    assert (tmp / "GLUE").read_text() == "kept"   # nothing changed
+    monkeypatch.setattr(build.importlib.metadata, "version", lambda name: "0.0")
+    build.build()
+    assert (tmp / "GLUE").read_text() == "one"
+
+
+@pytest.mark.parametrize("how", ["fails", "no compiler", "no torch"])
+def test_a_torch_side_that_cannot_be_built_leaves_the_library(glue_files, monkeypatch, capsys, how):
+    """The codec does without it; what was built of an older source is gone."""
+    build, tmp = glue_files
+    (tmp / "GLUE").write_text("old")
+
+    def no_torch(out):
+        raise RuntimeError("torch not found")
+
+    monkeypatch.setattr(build, "glue_command", {"fails": lambda out: ["false"], "no compiler": lambda out: [str(tmp / "none")], "no torch": no_torch}[how])
+    assert build.build() == build.LIB
+    assert not (tmp / "GLUE").exists() and "_glue.so" in capsys.readouterr().err
+
+
 def _rank(rank, world, port, queue):
     import os
 
