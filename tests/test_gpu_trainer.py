@@ -491,6 +491,60 @@ def test_masks_over_many_rows(crx, n):
     assert bool((grad.abs().sum(-1) != 0).cpu()[~mask].sum() == 0)
 
 
+@pytest.mark.parametrize("B,T,V,dtype", [
+    (1, 1300, 152064, torch.bfloat16),   # clusters whose rows do not fit the rings, about nine rows each
+    (2, 350, 33000, torch.float32),      # clusters of two
+    (1, 1300, 33001, torch.bfloat16),    # CTAs whose rows do not fit
+    (1, 1900, 12001, torch.bfloat16),    # CTAs whose rows do
+    (1, 1400, 12001, torch.float32),
+    (3, 2000, 4099, torch.float16),      # warps
+    (1, 5000, 9001, torch.bfloat16),     # warps whose rows do not fit
+], ids=str)
+@pytest.mark.parametrize("masked", [False, True], ids=["all", "masked"])
+def test_many_rows_that_count_for_every_unit(crx, B, T, V, dtype, masked):
+    """Rings, barriers and the parts of a cluster over many rows, row by row; equal bits when it runs again."""
+    g = torch.Generator(device="cuda").manual_seed(41)
+    z = (torch.randn(B, T, V, generator=g, device="cuda") * 2.5).to(dtype)
+    tokens = torch.randint(0, V, (B, T), generator=g, device="cuda")
+    z.scatter_add_(2, tokens[..., None], (torch.rand(B, T, 1, generator=g, device="cuda") * 9).to(dtype))
+    adv = torch.randn(B, T, generator=g, device="cuda")
+    mask = torch.rand(B, T, generator=g, device="cuda") < 0.8 if masked else torch.ones(B, T, dtype=torch.bool, device="cuda")
+    leaf = z.detach().requires_grad_()
+
+    def once():
+        out = crx.policy_loss(leaf, tokens, adv, mask=mask if masked else None)
+        return out, torch.autograd.grad(out.loss, leaf)[0]
+
+    out, grad = once()
+    u = (-adv.double() / mask.sum()) * mask
+    depth = V / 512 + 48
+    for b in range(B):
+        for lo in range(0, T, 50):
+            part = slice(lo, min(T, lo + 50))
+            q = torch.log_softmax(z[b, part].double(), -1)
+            a = tokens[b, part, None]
+            logp = q.gather(1, a)[:, 0]
+            on = mask[b, part]
+            tilt = (z[b, part].double().gather(1, a)[:, 0] - (q.exp() * z[b, part].double()).sum(-1)).abs()
+            tol = ref.H * (depth + 12 + 4 * logp.abs() + 2 * tilt + math.log(V))   # as in trainer_ref
+            assert bool(((out.logp[b, part].double() - torch.where(on, logp, 0.0)).abs() <= tol).all()), (b, lo)
+            p = q.exp()
+            hot = torch.zeros_like(p).scatter_(1, a, 1.0)
+            ub = u[b, part, None]
+            want = ub * (hot - p)
+            bound = ub.abs() * (8 * ref.H * (hot + p) + p * ref.H * (depth + 20 + 3 * q.abs() + 2 * math.log(V))) + ref.half_step(want, dtype)
+            assert bool(((grad[b, part].double() - want).abs() <= bound).all()), (b, lo)
+    loss = float((adv.double() * mask).sum() / -mask.sum())   # (every ratio is 1)
+    assert abs(float(out.loss.detach()) - loss) <= 4 * ref.H * float((adv.double().abs() * mask).sum() / mask.sum())
+    with torch.no_grad():
+        alone = crx.policy_loss(z, tokens, adv, mask=mask if masked else None)
+    # another split of the row, each within the tolerance (the tilt is at most |logp| + log V)
+    assert bool(((alone.logp - out.logp).abs().double() <= 2 * ref.H * (depth + 12 + 6 * out.logp.abs().double() + 3 * math.log(V))).all())
+    for _ in range(3):
+        out2, grad2 = once()
+        assert torch.equal(out2.logp, out.logp) and torch.equal(out2.loss, out.loss) and torch.equal(grad2, grad)
+
+
 def test_a_mask_that_leaves_nothing(crx):
     d = batch(2, 3, 100, torch.float32, 9, mask=torch.zeros(2, 3, dtype=torch.bool))
     out, grad = run(crx, d, kl_coef=0.04)
