@@ -12,7 +12,6 @@
 #include <torch/extension.h>
 
 #include <algorithm>
-#include <cstring>
 #include <new>
 #include <string>
 #include <utility>
@@ -284,6 +283,13 @@ Results run(Call& c, const at::Tensor& logits, bool want_grad) {
     return r;
 }
 
+// What the backward pass needs beside the saved tensors.
+struct Kept : torch::CustomClassHolder {
+    crx_policy_args a;
+    int64_t capture;        // the graph that the forward pass was captured into
+    at::Tensor rows, grad;   // grad: until it is handed out
+};
+
 // The graph that the device's current stream is being captured into, 0 for none.
 int64_t capture_of(int dev) {
     cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
@@ -301,10 +307,12 @@ struct PolicyLossFn : public torch::autograd::Function<PolicyLossFn> {
         Results r = run(*c, logits, true);
         const auto stats = r.stats.unbind(0);
         ctx->save_for_backward({logits, c->tokens});
-        ctx->saved_data["args"] = std::string(reinterpret_cast<const char*>(&c->a), sizeof c->a);
-        ctx->saved_data["rows"] = r.rows;
-        ctx->saved_data["grad"] = r.grad;
-        ctx->saved_data["capture"] = capture_of(c->dev);
+        auto keep = c10::make_intrusive<Kept>();
+        keep->a = c->a;
+        keep->capture = capture_of(c->dev);
+        keep->rows = std::move(r.rows);
+        keep->grad = std::move(r.grad);
+        ctx->saved_data["kept"] = c10::IValue::make_capsule(std::move(keep));
         ctx->mark_non_differentiable({r.logp, stats[0], stats[1]});
         ctx->set_materialize_grads(false);
         return {r.loss, r.logp, stats[0], stats[1]};
@@ -315,25 +323,18 @@ struct PolicyLossFn : public torch::autograd::Function<PolicyLossFn> {
         if (!scale.defined()) return {at::Tensor(), at::Tensor()};
         const auto saved = ctx->get_saved_variables();   // refuses tensors modified since
         const at::Tensor &logits = saved[0], &tokens = saved[1];
-        crx_policy_args a;
-        std::memcpy(&a, ctx->saved_data["args"].toStringRef().data(), sizeof a);
-        const at::Tensor rows_kept = ctx->saved_data["rows"].toTensor();
-        const int dev = rows_kept.get_device();
+        const auto capsule = ctx->saved_data["kept"].toCapsule();
+        Kept& kept = static_cast<Kept&>(*capsule);
+        crx_policy_args a = kept.a;
+        const int dev = kept.rows.get_device();
         TORCH_CHECK(same_again(logits, tokens, dev, a) && rows(tokens, tokens, false, &a.tokens),
                     "policy_loss: saved logits or tokens came back with another shape, type or device");
         const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
-        c10::IValue& kept = ctx->saved_data["grad"];
-        at::Tensor grad;
-        const bool first = kept.isTensor() && ctx->saved_data["capture"].toInt() == capture_of(dev);
-        if (first) {
-            grad = kept.toTensor();
-            kept = c10::IValue();
-        } else {
-            grad = grad_like(logits);
-        }
+        const bool first = kept.grad.defined() && kept.capture == capture_of(dev);
+        const at::Tensor grad = first ? std::exchange(kept.grad, at::Tensor()) : grad_like(logits);
         a.logits = wide_rows(logits);
         a.grad = wide_rows(grad);
-        a.rows = static_cast<float*>(rows_kept.data_ptr());
+        a.rows = static_cast<float*>(kept.rows.data_ptr());
         a.logp = a.loss = a.stats = a.rows;   // results that this pass does not touch
         char err[512] = "";
         const int st = crx_policy_backward(&a, scale.data_ptr<float>(), first, stream_of(dev), err, sizeof err);
