@@ -3,7 +3,7 @@
 //
 // Per row of V logits, in units of log2 (c = log2(e) / temperature):
 //   M = max z, R = M c, s = sum 2^(z c - R)        one pass, the maximum kept as it goes
-//   logp = (z_a c - R - log2 s) ln 2
+//   logp = (z_a - M) / temperature - ln(s 2^(R - M c))      (R is M c rounded to fp32)
 //   d loss / d z_j = u (1[j = a] - 2^(z_j c - R) / s),  u = w / D / temperature * d l / d logp
 // u depends on the row's own logp alone (D is known before), so the gradient is written in the
 // same visit to the row: the logits are read from HBM once and written once.
@@ -583,7 +583,10 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) k_policy_rows(const __g
         const bool far = fabsf(run.m) <= 3.402823466e38f && !(fabsf(run.m * c) < kFar);
         const float s = far ? far_sum<T, WARP>(z, V, run.m, c, sh) : run.s;
         const float R = far ? run.m : run.r;
-        const float logp = ((far ? (za - R) * c : fmaf(za, c, -R)) - log2f(s)) * 0.6931471805599453f;
+        // the token's term from the logits themselves (halved: their difference may not fit), not through c's
+        // rounding; s without what the maximum's exponent is off 0
+        const float at_top = far ? s : s * exp2_fast(-fmaf(run.m, c, -R));
+        const float logp = (0.5f * za - 0.5f * run.m) / (0.5f * a.temperature) - logf(at_top);
 
         const float A = r.advantage;
         const float ratio = a.old_logp.p ? expf(logp - r.old) : (logp == logp ? 1.f : logp);   // NaN logits show in the loss

@@ -434,6 +434,19 @@ def test_policy_loss_of_a_broadcast_leaf(crx):
     near(leaf.grad, want["grad"].sum((0, 1), keepdim=True), want["tol_grad"].sum((0, 1), keepdim=True) + 12 * ref.H * want["grad"].abs().sum((0, 1), keepdim=True))
 
 
+@pytest.mark.parametrize("tau,roundings", [(1.0, 1), (0.75, 2)])
+def test_log_probabilities_of_unlikely_tokens(crx, tau, roundings):
+    """Next to one large logit: the difference of two logits, which bf16 ones have exactly, over the temperature."""
+    z = torch.zeros(4000, 2, dtype=torch.bfloat16)
+    z[:, 0] = torch.rand(4000, generator=gen(44)) * 100 - 40
+    z[:, 1] = z[:, 0].float() - 18 - torch.rand(4000, generator=gen(45)) * 40
+    tokens = torch.ones(4000, dtype=torch.int64)
+    out = crx.policy_loss(z.cuda(), dev(tokens), torch.ones(4000, device="cuda"), temperature=tau)
+    want = torch.log_softmax(z.double() / tau, -1)[:, 1]
+    # the quotient (exact where it is by 1) and the sum with log s are rounded; s is 1 to e^-18 + H, twice that in 2^x
+    near(out.logp, want, roundings * ref.H * want.abs() + 2 * (math.exp(-17) + ref.H))
+
+
 def test_policy_loss_of_one_sequence(crx):
     d = batch(1, 23, 999, torch.float16, 6)
     one = {k: v[0] if torch.is_tensor(v) else v for k, v in d.items()}
