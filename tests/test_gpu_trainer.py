@@ -2,6 +2,7 @@
 sizes, layouts, masks and values where they can go wrong, and run together as a trainer does."""
 
 import contextlib
+import gc
 import math
 
 import pytest
@@ -21,6 +22,13 @@ def _gpu():
         pytest.skip("needs a CUDA GPU")
     from crukx_sync_b200 import _ext
     _ext.load()
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _collected():
+    """No tensors stay behind in reference cycles (a graphed callable is one): a later test counts memory."""
+    yield
+    gc.collect()
 
 
 @pytest.fixture(scope="module")
