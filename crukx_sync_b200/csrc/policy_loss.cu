@@ -17,10 +17,10 @@
 //   k_policy_sums    one CTA: the terms of the rows summed in a fixed order, in double
 //   k_policy_again   the gradient once more, scaled, from the rows' saved (u, R, s)
 //
-// Bounds: HBM where nothing interferes (without gradient 4096 x 152k rows, 894 MB that count, take
-// 0.142 ms, 6.3 TB/s; with it 2143 MB 0.38 ms, 5.6 TB/s).  What is left between that and the 6.5 of a
-// copy: rows that do not fit the rings come through L2 twice (without the second time 0.36 ms), and the
-// CTAs of a cluster wait for one another once a row.  Leaving the exponentials out changes nothing.
+// Bounds: HBM (without gradient 4096 x 152k rows, 894 MB that count, take 0.17 ms, 5.2 TB/s; with it
+// 2143 MB 0.42 ms, 5.1 TB/s; a copy does 6.5).  What is left: rows that do not fit the rings come through
+// L2 twice (5 % of it), the CTAs of a cluster wait for one another once a row, and the plan and the sums.
+// Leaving the exponentials out changes nothing.  The second pass of a scaled loss takes 0.46 ms.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -42,8 +42,8 @@ namespace {
 namespace cg = cooperative_groups;
 
 // Sixteen warps per SM in CTAs of four, whose reductions pass under one another's streams: 4096 x 152k
-// rows with their gradient take 0.38 ms, by CTAs of two warps 0.39, of sixteen 0.40; with 24 or 32 warps
-// per SM and shorter rings 0.45 and 0.48.  Rings fill what shared memory there is.
+// rows with their gradient take 0.42 ms, by CTAs of two warps 0.43, of sixteen 0.44; with 24 or 32 warps
+// per SM and shorter rings 0.50 and 0.54.  Rings fill what shared memory there is.
 constexpr int kRowThreads = 128;
 constexpr int kRowWarps = kRowThreads / 32;
 constexpr int kMaxCluster = 8;
@@ -752,8 +752,8 @@ int fail(char* err, size_t errlen, int status, const std::string& msg) {
 
 // A row that does not fit the rings is read a second time for its gradient, out of L2 as long as the
 // rows that are being worked on at once are no more than this (of 126 MB; the gradients pass through
-// it too).  4096 x 152k bf16 rows, 28% of them masked: 0.38 ms with 48 MB, 0.41 with 24 (more CTAs per
-// row wait for one another), 0.48 with 96; 2048 x 152k fp32: 0.45, 0.44, 0.55.
+// it too).  4096 x 152k bf16 rows, 28% of them masked: 0.42 ms with 48 MB, 0.47 with 24 (more CTAs per
+// row wait for one another), 0.52 with 96; 2048 x 152k fp32: 0.38, 0.38, 0.46.
 constexpr int64_t kRowsAtOnce = int64_t(48) << 20;
 
 // A row by one warp, where nothing waits for another warp: rows short enough, and as many of them as

@@ -13,7 +13,7 @@ as encode_update takes its weights.  Every call runs on the tensors' device and 
 waits for nothing, and takes its scratch from torch's allocator, so calls on different streams do
 not meet and a call can be captured into a CUDA graph.  In a captured graph the Python numbers
 among the arguments are fixed; adamw_step's `lr` and `step` may be tensors that it reads when it
-runs.  Caller mistakes are ValueErrors, raised before anything is launched.
+runs.  Numbers are taken in fp32, and refused where they would be 0 or infinite there.  Caller mistakes are ValueErrors, raised before anything is launched.
 """
 
 from __future__ import annotations
@@ -144,8 +144,9 @@ def clip_grads(grads: Mapping[str, torch.Tensor], max_norm: float, *, out: Mappi
     Every gradient is multiplied by min(1, max_norm / (norm + 1e-6)) and rounded to its type: in
     place, or into the tensors of `out` (same names, sizes and types).  `norm` (0-d fp32, on the
     device) takes the place of the gradients' own, for gradients spread over ranks
-    (dist.grad_norm_global).  A norm that is not finite is not clipped away: it leaves NaN, as its
-    product says.  Tensors that share memory (a tied weight under two names) are refused."""
+    (dist.grad_norm_global).  A norm that is not finite is not clipped away: NaN leaves NaN, and an
+    infinite one 0, or NaN where the gradient is infinite, as the products say.  Tensors that share
+    memory (a tied weight under two names) are refused."""
     max_norm = _real("max_norm", max_norm)
     if not max_norm >= _LEAST:   # (NaN too)
         raise ValueError(f"max_norm must be positive (in fp32), got {max_norm}")

@@ -294,7 +294,8 @@ typedef struct crx_adamw_args {
     float max_norm;          /* > 0: gradients are scaled by min(1, max_norm / (*norm + 1e-6)) on the way */
 } crx_adamw_args;
 /* AdamW with decoupled weight decay on fp32 masters and moments, in place; weights[i] (weights may
- * be NULL) receives the bf16 rounding of master i.  Memory that is written may not be shared. */
+ * be NULL) receives the bf16 rounding of master i.  Memory that is written may not be shared.  Numbers
+ * are taken in fp32: an eps that is 0 there, an lr or weight_decay that is not finite, is CRX_VALUE_ERROR. */
 int crx_adamw_step(int32_t n_tensors, float* const* master, const void* const* grads, const int32_t* dtypes,
                    float* const* exp_avg, float* const* exp_avg_sq, void* const* weights, const int64_t* numel,
                    const crx_adamw_args* args, void* stream, char* err, size_t errlen);
@@ -327,7 +328,8 @@ int64_t crx_policy_workspace(int64_t batch, int64_t steps);
  *   l = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^x - x - 1), x = ref_logp - logp
  * loss = sum w l / denom; KL and clipped fraction are averaged the same way.  Tokens with w = 0 are
  * left out whatever their values: logp 0, gradient 0, logits not read.  denom = 0 in effect (an
- * all-zero mask) gives 0.  A token outside the vocabulary where w != 0 makes the loss NaN. */
+ * all-zero mask) gives 0.  A token outside the vocabulary where w != 0 makes the loss NaN, whatever its
+ * advantage. */
 int crx_policy_loss(const crx_policy_args* args, void* stream, char* err, size_t errlen);
 /* grad = scale * the gradient that crx_policy_loss wrote (args as it got them; scale: device
  * scalar).  unless_one != 0: nothing is done where *scale is 1 (grad holds the answer already). */
